@@ -538,8 +538,10 @@ const char *sp_cuda_last_error_string(void);
 
 /* New: sizeof(sp_config_t) (which=0), sizeof(sp_band_config_t) (1),
  * sizeof(sp_cuda_cache_t) (2), sizeof(sp_cuda_sqfree_cache_t) (3),
- * sizeof(sp_cuda_hier_cache_t) (4), sizeof(sp_cuda_cold_layer_t) (5), so
- * bindings can check their mirrors. */
+ * sizeof(sp_cuda_hier_cache_t) (4), sizeof(sp_cuda_cold_layer_t) (5), and of
+ * shannon_prime_q8.h sizeof(sp_cuda_q8_cache_t) (6),
+ * sizeof(sp_cuda_q8_batch_t) (7), sizeof(sp_rope_axes_t) (8), so bindings can
+ * check their mirrors. */
 int sp_cuda_abi_struct_size(int which);
 
 /* New, for tests and benchmarks: force the fused-decode kernel family

@@ -1,6 +1,7 @@
 // sp_api.cu — cache lifecycle and the reference-named write/read entry
 // points of shannon_prime_cuda.h, plus the per-thread status of the C-ABI.
 #include "sp_internal.cuh"
+#include "shannon_prime_q8.h"
 
 #include <math.h>
 #include <stdarg.h>
@@ -278,7 +279,7 @@ extern "C" void sp_cuda_read_v_batch(const sp_cuda_cache_t *cc, int layer, int h
 
 // sizeof of the public structs, so bindings in other languages can check
 // their mirror of the layout (0 = sp_config_t, 1 = sp_band_config_t,
-// 2 = sp_cuda_cache_t).
+// 2 = sp_cuda_cache_t, ...).
 extern "C" int sp_cuda_abi_struct_size(int which)
 {
     switch (which) {
@@ -288,6 +289,9 @@ extern "C" int sp_cuda_abi_struct_size(int which)
     case 3: return (int)sizeof(sp_cuda_sqfree_cache_t);
     case 4: return (int)sizeof(sp_cuda_hier_cache_t);
     case 5: return (int)sizeof(sp_cuda_cold_layer_t);
+    case 6: return (int)sizeof(sp_cuda_q8_cache_t);
+    case 7: return (int)sizeof(sp_cuda_q8_batch_t);
+    case 8: return (int)sizeof(sp_rope_axes_t);
     }
     return -1;
 }

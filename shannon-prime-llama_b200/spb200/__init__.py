@@ -1,5 +1,5 @@
 """ctypes binding of the B200 Shannon-Prime C-ABI (include/shannon_prime_cuda.h,
-include/shannon_prime_llama.h).
+include/shannon_prime_llama.h, include/shannon_prime_q8.h).
 
 The library is the in-tree lib/libshannon_prime_b200.so built by
 shannon-prime-llama_b200/build.py.  There is no fallback: if the library is
@@ -21,6 +21,10 @@ LIB_PATH = Path(os.environ["SPB200_LIB"]) if os.environ.get("SPB200_LIB") else P
 SP_MAX_BANDS = 16
 SP_OK, SP_ERR_ARG, SP_ERR_CUDA, SP_ERR_UNSUPPORTED, SP_ERR_TIMEOUT = 0, -1, -2, -3, -4
 SP_DTYPE_F32, SP_DTYPE_F16, SP_DTYPE_BF16 = 0, 1, 2
+SP_MAX_HEAD_DIM = 512
+SP_Q8_INT8, SP_Q8_E4M3 = 0, 1
+SP_ROPE_ADJACENT, SP_ROPE_HALVES = 0, 1
+SP_ROPE_INTERLEAVED, SP_ROPE_AXIS_LADDER = 1, 2
 
 
 class SpConfig(C.Structure):
@@ -101,6 +105,30 @@ class SpColdLayer(C.Structure):
         ("h_pinned", C.c_void_p), ("capacity", C.c_int64), ("packed_stride", C.c_int),
         ("n_heads", C.c_int), ("write_head", C.c_int64), ("oldest_pos", C.c_int64),
         ("newest_pos", C.c_int64), ("ring_mode", C.c_bool), ("initialized", C.c_bool),
+    ]
+
+
+class SpQ8Cache(C.Structure):
+    _fields_ = [
+        ("config", SpConfig), ("format", C.c_int), ("block_tokens", C.c_int), ("n_seqs", C.c_int),
+        ("max_seq_len", C.c_int), ("d_k_cache", C.c_void_p), ("d_v_cache", C.c_void_p),
+        ("d_k_scale", C.c_void_p), ("d_v_scale", C.c_void_p), ("stream", C.c_void_p),
+        ("n_slots", C.c_int), ("device", C.c_int), ("sm_count", C.c_int),
+        ("d_attn_ws", C.c_void_p), ("attn_ws_bytes", C.c_size_t), ("d_status", C.c_void_p),
+    ]
+
+
+class SpQ8Batch(C.Structure):
+    _fields_ = [
+        ("n_seqs", C.c_int), ("n_tokens", C.c_int), ("max_new", C.c_int), ("max_kv", C.c_int),
+        ("d_seq", C.c_void_p), ("d_cu", C.c_void_p), ("d_kv_len", C.c_void_p),
+    ]
+
+
+class SpRopeAxes(C.Structure):
+    _fields_ = [
+        ("head_dim", C.c_int), ("rot_dim", C.c_int), ("n_axes", C.c_int), ("pairing", C.c_int),
+        ("phase", C.c_uint64 * (SP_MAX_HEAD_DIM // 2)), ("axis", C.c_uint8 * (SP_MAX_HEAD_DIM // 2)),
     ]
 
 
@@ -203,6 +231,18 @@ SIGNATURES = {
     "sp_cuda_attn_profile": (_V, [_I]),
     "sp_cuda_attn_last_kernel_ms": (_F, []),
     "sp_cuda_attn_last_splits": (_I, []),
+    # shannon_prime_q8.h
+    "sp_rope_axes_init": (_I, [C.POINTER(SpRopeAxes), _I, _I, _I, _I, C.POINTER(C.c_int), _I, C.c_double,
+                               C.POINTER(C.c_float)]),
+    "sp_cuda_rope_axes": (_I, [C.POINTER(SpRopeAxes), _P, _I, _P, C.c_longlong, _I, _P, C.c_longlong, _P,
+                               C.c_longlong, _I, _P, C.c_longlong, _I, _I, _P]),
+    "sp_cuda_q8_cache_init": (_I, [C.POINTER(SpQ8Cache), C.POINTER(SpConfig), _I, _I, _I, _I, _P]),
+    "sp_cuda_q8_cache_free": (_V, [C.POINTER(SpQ8Cache)]),
+    "sp_cuda_q8_write_kv_tokens": (_I, [C.POINTER(SpQ8Cache), _I, C.POINTER(SpQ8Batch), _P, _P, C.c_longlong, _I]),
+    "sp_cuda_q8_read_kv_tokens": (_I, [C.POINTER(SpQ8Cache), _I, _I, _I, _I, _I, _P, _I]),
+    "sp_cuda_q8_attn": (_I, [C.POINTER(SpQ8Cache), _I, C.POINTER(SpQ8Batch), _P, C.c_longlong, _I, _I, _F, _I, _I, _P,
+                             C.c_longlong, _P, _P]),
+    "sp_cuda_q8_status": (_I, [C.POINTER(SpQ8Cache), C.POINTER(C.c_uint), _I, _P]),
     # shannon_prime_llama.h
     "sp_llama_init": (_P, [C.POINTER(SpLlamaParams)]),
     "sp_llama_init_with_role": (_P, [C.POINTER(SpLlamaParams), _I]),
@@ -249,7 +289,9 @@ def lib() -> C.CDLL:
             f.restype = res
             f.argtypes = args
         for which, st in enumerate((SpConfig, SpBandConfig, SpCudaCache, SpSqfreeCache, SpHierCache,
-                                     SpColdLayer)):
+                                     SpColdLayer, SpQ8Cache, SpQ8Batch, SpRopeAxes)):
+            if which > 5 and os.environ.get("SPB200_LIB") and not hasattr(L, "sp_cuda_q8_attn"):
+                continue
             if L.sp_cuda_abi_struct_size(which) != C.sizeof(st):
                 raise RuntimeError(f"struct mirror {st.__name__} does not match the C ABI")
         _lib = L
@@ -295,3 +337,4 @@ def _stream_ptr(stream) -> int:
 
 
 from .cache import Cache  # noqa: E402,F401
+from .q8 import Q8Batch, Q8Cache, RopeAxes  # noqa: E402,F401

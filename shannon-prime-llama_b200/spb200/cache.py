@@ -85,12 +85,14 @@ class Cache:
         check(rc, "sp_cuda_attn_decode")
 
 
-def _wrap_device(ptr: int, nbytes: int, dtype):
-    """A torch CUDA tensor aliasing nbytes of device memory at ptr."""
+def _wrap_device(ptr: int, nbytes: int, dtype, owner=None):
+    """A torch CUDA tensor aliasing nbytes of device memory at ptr; the tensor
+    keeps `owner`, whose memory it is, alive."""
     import torch
 
     class _Holder:
         def __init__(self, p, n):
+            self.owner = owner
             self.__cuda_array_interface__ = {
                 "shape": (n,), "typestr": "|u1", "data": (p, False), "version": 3}
 

@@ -1,0 +1,195 @@
+"""Python mirror of the 8-bit cache (shannon_prime_q8.h): rotary positions
+with several axes, the quantising write, the read back and attention.  Every
+method calls straight into the C-ABI; device buffers are torch CUDA tensors."""
+from __future__ import annotations
+
+import ctypes as C
+
+from . import (SP_DTYPE_BF16, SP_DTYPE_F16, SP_DTYPE_F32, SP_Q8_E4M3, SP_Q8_INT8, SP_ROPE_ADJACENT,
+               SP_ROPE_AXIS_LADDER, SP_ROPE_HALVES, SP_ROPE_INTERLEAVED, SpConfig, SpQ8Batch, SpQ8Cache, SpRopeAxes,
+               _ptr, _stream_ptr, check, lib)
+from .cache import _wrap_device
+
+_FORMATS = {"int8": SP_Q8_INT8, "e4m3": SP_Q8_E4M3}
+_PAIRINGS = {"adjacent": SP_ROPE_ADJACENT, "halves": SP_ROPE_HALVES}
+_DTYPES: dict = {}
+
+
+def _dtype(t) -> int:
+    if not _DTYPES:
+        import torch
+        _DTYPES.update({torch.float32: SP_DTYPE_F32, torch.float16: SP_DTYPE_F16, torch.bfloat16: SP_DTYPE_BF16})
+    code = _DTYPES.get(t.dtype)
+    if code is None:
+        raise TypeError(f"{t.dtype}: float32, float16 and bfloat16 are possible")
+    return code
+
+
+def _rows(t, heads, head_dim: int, what: str) -> int:
+    """The token stride of t [n_tokens][heads][head_dim], whose rows lie together."""
+    if t.dim() != 3 or t.shape[2] != head_dim or (heads is not None and t.shape[1] != heads):
+        raise ValueError(f"{what}: shape {tuple(t.shape)}, not [tokens][{heads or 'heads'}][{head_dim}]")
+    s = t.stride()
+    if not t.is_cuda or (t.numel() and (s[2] != 1 or (t.shape[1] > 1 and s[1] != head_dim))):
+        raise ValueError(f"{what}: a token's heads must lie together in device memory")
+    return s[0] if t.shape[0] > 1 else 0
+
+
+class RopeAxes:
+    """A rotation plan: `sections` pairs for each axis (together rot_dim / 2)."""
+
+    def __init__(self, head_dim: int, sections, rot_dim: int | None = None, pairing: str = "adjacent",
+                 interleave: bool = False, axis_ladder: bool = False, theta: float = 10000.0, freq_factors=None):
+        sections = [int(n) for n in sections]
+        rot_dim = 2 * sum(sections) if rot_dim is None else rot_dim
+        self.plan = SpRopeAxes()
+        flags = (SP_ROPE_INTERLEAVED if interleave else 0) | (SP_ROPE_AXIS_LADDER if axis_ladder else 0)
+        ff = None if freq_factors is None else (C.c_float * (rot_dim // 2))(*freq_factors)
+        check(lib().sp_rope_axes_init(C.byref(self.plan), head_dim, rot_dim, _PAIRINGS[pairing], len(sections),
+                                      (C.c_int * len(sections))(*sections), flags, theta, ff), "sp_rope_axes_init")
+        self.head_dim, self.n_axes = head_dim, len(sections)
+        self._ref, self._call = C.byref(self.plan), lib().sp_cuda_rope_axes
+
+    def apply(self, pos, q=None, k=None, q_out=None, k_out=None, inverse: bool = False, stream=None):
+        """Rotates q and k ([tokens][heads][head_dim] CUDA tensors; either may be
+        None) at positions pos (int32 [axes][tokens]).  The outputs are new
+        tensors unless given; an output may be its input.  Returns both."""
+        import torch
+        t = q if q is not None else k
+        n = 0 if t is None else t.shape[0]
+        if pos.dtype != torch.int32 or tuple(pos.shape) != (self.n_axes, n) or not pos.is_contiguous() or not pos.is_cuda:
+            raise ValueError(f"pos must be a contiguous int32 CUDA tensor [{self.n_axes}][{n}]")
+        a, dt = [], 0
+        for name, x, y in (("q", q, q_out), ("k", k, k_out)):
+            if x is None:
+                a.append((0, 0, 0, 0, 0))
+                continue
+            if y is None:
+                y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            if name == "q":
+                q_out = y
+            else:
+                k_out = y
+            if x.shape[0] != n or y.shape != x.shape or y.dtype != x.dtype or x.dtype != t.dtype:
+                raise ValueError(f"{name}: inputs and outputs must have one type and {n} tokens")
+            dt = _dtype(x)
+            a.append((x.data_ptr(), _rows(x, None, self.head_dim, name), x.shape[1], y.data_ptr(),
+                      _rows(y, None, self.head_dim, name)))
+        (qp, qs, hq, qo, qos), (kp, ks, hk, ko, kos) = a
+        rc = self._call(self._ref, pos.data_ptr(), n, qp, qs, hq, qo, qos, kp, ks, hk, ko, kos, dt, int(inverse),
+                        _stream_ptr(stream))
+        if rc:
+            check(rc, "sp_cuda_rope_axes")
+        return q_out, k_out
+
+
+class Q8Batch:
+    """The new tokens of one step: cu [n + 1] and kv_len [n] (and seq [n], where
+    the entries are not sequences 0, 1, ...), int32 CUDA tensors; n_tokens packed
+    tokens, at most max_new of one entry, at most max_kv positions held."""
+
+    def __init__(self, cu, kv_len, n_tokens: int, max_new: int, max_kv: int, seq=None):
+        import torch
+        n = kv_len.shape[0]
+        for name, t, size in (("cu", cu, n + 1), ("kv_len", kv_len, n), ("seq", seq, n)):
+            if t is not None and (t.dtype != torch.int32 or tuple(t.shape) != (size,) or not t.is_contiguous()
+                                  or not t.is_cuda):
+                raise ValueError(f"{name} must be a contiguous int32 CUDA tensor [{size}]")
+        self._keep = (cu, kv_len, seq)
+        self.n_tokens = n_tokens
+        self.b = SpQ8Batch(n, n_tokens, max_new, max_kv, _ptr(seq), cu.data_ptr(), kv_len.data_ptr())
+        self.ref = C.byref(self.b)
+
+
+class Q8Cache:
+    """A cache held in 8 bits (sp_cuda_q8_cache_t) on the current device.  Writes
+    and reads are ordered on `stream`, attention on the stream it is given."""
+
+    def __init__(self, head_dim: int, n_layers: int, n_heads_kv: int, max_seq_len: int, n_seqs: int = 1,
+                 fmt: str = "int8", block_tokens: int = 64, stream=None):
+        self.qc = SpQ8Cache()
+        self.stream, self.fmt = stream, fmt
+        cfg = SpConfig(head_dim=head_dim, n_layers=n_layers, n_heads_kv=n_heads_kv)
+        check(lib().sp_cuda_q8_cache_init(C.byref(self.qc), C.byref(cfg), _FORMATS[fmt], block_tokens, n_seqs,
+                                          max_seq_len, _stream_ptr(stream)), "sp_cuda_q8_cache_init")
+        self.head_dim, self.n_layers, self.n_heads_kv, self.n_seqs = head_dim, n_layers, n_heads_kv, n_seqs
+        self.block_tokens, self.max_seq_len = block_tokens, self.qc.max_seq_len
+        self._ref = C.byref(self.qc)
+        self._write, self._read, self._attn = (lib().sp_cuda_q8_write_kv_tokens, lib().sp_cuda_q8_read_kv_tokens,
+                                               lib().sp_cuda_q8_attn)
+
+    def free(self) -> None:
+        if self.qc.d_k_cache:
+            lib().sp_cuda_q8_cache_free(C.byref(self.qc))
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+    def slab(self, which: int):
+        """The K (0) or V (1) codes [layers][seqs][heads][max_seq_len][head_dim]
+        (int8 or float8_e4m3fn; shares memory with the cache and keeps it)."""
+        import torch
+        shape = (self.n_layers, self.n_seqs, self.n_heads_kv, self.max_seq_len, self.head_dim)
+        n = self.qc.n_slots * self.max_seq_len * self.head_dim
+        t = torch.int8 if self.fmt == "int8" else torch.float8_e4m3fn
+        return _wrap_device(self.qc.d_v_cache if which else self.qc.d_k_cache, n, t, self).view(shape)
+
+    def scales(self, which: int):
+        """The scales [layers][seqs][heads][blocks] (shares memory with the cache and keeps it)."""
+        import torch
+        shape = (self.n_layers, self.n_seqs, self.n_heads_kv, self.max_seq_len // self.block_tokens)
+        n = self.qc.n_slots * shape[-1] * 4
+        return _wrap_device(self.qc.d_v_scale if which else self.qc.d_k_scale, n, torch.float32, self).view(shape)
+
+    def write_kv_tokens(self, layer: int, batch: Q8Batch, k, v) -> None:
+        """k, v: [n_tokens][n_heads_kv][head_dim] (f32/f16/bf16, one token stride;
+        either may be None)."""
+        t = k if k is not None else v
+        if t is None:
+            return
+        stride = _rows(t, self.n_heads_kv, self.head_dim, "k")
+        if k is not None and v is not None and (v.dtype != k.dtype or _rows(v, self.n_heads_kv, self.head_dim, "v") != stride
+                                                or v.shape[0] != k.shape[0]):
+            raise ValueError("k and v must have one type, token stride and number of tokens")
+        if t.shape[0] != batch.n_tokens:
+            raise ValueError(f"{t.shape[0]} tokens, the batch has {batch.n_tokens}")
+        rc = self._write(self._ref, layer, batch.ref, 0 if k is None else k.data_ptr(), 0 if v is None else v.data_ptr(),
+                         stride, _dtype(t))
+        if rc:
+            check(rc, "sp_cuda_q8_write_kv_tokens")
+
+    def read_kv_tokens(self, which: int, layer: int, seq: int, start_pos: int, out) -> None:
+        """out: [n_tok][n_heads_kv][head_dim], contiguous (f32/f16/bf16)."""
+        if not out.is_contiguous() or tuple(out.shape[1:]) != (self.n_heads_kv, self.head_dim):
+            raise ValueError(f"out must be contiguous [tokens][{self.n_heads_kv}][{self.head_dim}]")
+        rc = self._read(self._ref, which, layer, seq, start_pos, out.shape[0], out.data_ptr(), _dtype(out))
+        if rc:
+            check(rc, "sp_cuda_q8_read_kv_tokens")
+
+    def attn(self, layer: int, batch: Q8Batch, q, out=None, lse=None, logit_scale: float = 1.0, causal: bool = True,
+             window: int = 0, stream=None):
+        """q: [n_tokens][n_q_heads][head_dim] fp16 or bf16; out the same (new unless
+        given); lse: fp32 [n_tokens][n_q_heads] or None.  Returns out."""
+        import torch
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        qs, os = _rows(q, None, self.head_dim, "q"), _rows(out, q.shape[1], self.head_dim, "out")
+        n, hq = q.shape[0], q.shape[1]
+        if n != batch.n_tokens or out.shape[0] != n or out.dtype != q.dtype:
+            raise ValueError(f"q and out must have one type and the batch's {batch.n_tokens} tokens")
+        if lse is not None and (lse.dtype != torch.float32 or tuple(lse.shape) != (n, hq) or not lse.is_contiguous()):
+            raise ValueError(f"lse must be a contiguous float32 tensor [{n}][{hq}]")
+        rc = self._attn(self._ref, layer, batch.ref, q.data_ptr(), qs, hq, _dtype(q), logit_scale, int(causal), window,
+                        out.data_ptr(), os, 0 if lse is None else lse.data_ptr(), _stream_ptr(stream))
+        if rc:
+            check(rc, "sp_cuda_q8_attn")
+        return out
+
+    def status(self, clear: bool = False, stream=None) -> int:
+        """The device error word after the stream's work (synchronises)."""
+        v = C.c_uint(0)
+        check(lib().sp_cuda_q8_status(self._ref, C.byref(v), int(clear), _stream_ptr(stream)), "sp_cuda_q8_status")
+        return v.value
