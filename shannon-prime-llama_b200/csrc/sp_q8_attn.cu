@@ -1,92 +1,528 @@
-// sp_q8_attn.cu — attention over the 8-bit cache (shannon_prime_q8.h).
-#include "sp_q8.cuh"
+// sp_q8_attn.cu — attention over the 8-bit cache (shannon_prime_q8.h): the
+// entry point and the kernel for few rows (single tokens, draft tokens).
+#include "sp_q8_attn.cuh"
 
 #include <math.h>
 
-namespace q8 {
-size_t attn_workspace_bytes(int sm_count, int head_dim)
-{
-    (void)sm_count;
-    (void)head_dim;
-    return 256;
-}
-}  // namespace q8
+#include <atomic>
 
 namespace {
 
-struct AttnArgs {
-    q8::Layer l;
-    q8::Batch b;
-    const void *q;
-    void *out;
-    float *lse;
-    long long q_stride, out_stride;
-    int n_q_heads, group;
-    float scale;
-    int causal, window;
+using namespace q8;
+
+constexpr int kWarps = 8, kThreads = 32 * kWarps;
+constexpr int kTile = 16 * kWarps;       // positions of a tile: 16 for each warp
+
+__device__ __forceinline__ uint4 ldg16(const uint8_t *p)
+{
+    uint4 v;
+    asm("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint2 ldg8(const uint8_t *p)
+{
+    uint2 v;
+    asm("ld.global.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+    return v;
+}
+
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x)
+{
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+// Tiles of one (entry, KV head): the positions that any of its rows sees, from
+// a multiple of 16 on.  At least one, so that rows that see nothing are written.
+struct Unit0 {
+    int start, end, tiles;
+};
+__device__ __forceinline__ Unit0 unit_of(const AttnArgs &a, const Entry &e)
+{
+    Unit0 u = {0, e.kv_len, 0};
+    if (e.n <= 0 || (long long)e.n * a.group > a.few_rows) return u;
+    const int first = e.kv_len - e.n;
+    if (a.window > 0 && first - a.window + 1 > 0) u.start = (first - a.window + 1) & ~15;
+    u.tiles = max(1, (u.end - u.start + kTile - 1) / kTile);
+    return u;
+}
+
+template <int HD, int NT>
+struct FewSmem {
+    uint2 q[NT][HD / 16][32];                 // query fragments, one 8-byte word a lane
+    float up[8 * NT];                         // 2^exponent of each row
+    float m[kWarps][8 * NT], l[kWarps][8 * NT];
+    float o[4][8 * NT][HD + 4];               // + 4: rows on different banks
+    unsigned scan[kWarps], found[3];
+    int last;
 };
 
-// One warp for each (token, query head): one pass over the positions that the
-// token sees with a running maximum and sum, a lane holding every 32nd
-// element of the head.
-template <typename T, int FMT, int HD>
-__global__ void __launch_bounds__(128) k_q8_attn_rows(const __grid_constant__ AttnArgs a)
+// Rows of a unit are its new tokens times the query heads that share the KV
+// head, up to 8 NT of them.  A warp takes 16 positions at a time and works on
+// the transposed problem, S' = K q' and O' += V' P, so that positions and head
+// dimensions fill the 16-row side of mma.sync.m16n8k16 and the few rows its
+// 8-column side.  Codes go from memory to registers in the order in which the
+// fragments need them (a dimension's place in the product is free as long as
+// the queries have the same), become fp16 there, exactly, and meet fp16
+// queries scaled by a power of two to fit.  The score fragment becomes the
+// weight fragment by one movmatrix.
+//
+// Softmax in base 2 with the block's V scale folded into the exponent: weights
+// are w = 2^(s + log2 vs - m), m a running maximum of s + log2 vs (raised only
+// when a score passes it by 2^8, so w <= 2^8 and seldom rescaled); they are
+// rounded to fp16 for the product alone, relative to what they contribute,
+// and the sum of the unscaled weights is kept beside them in 32 bits as
+// sum w / vs.
+template <typename T, int FMT, int HD, int NT, int CTAS>
+__global__ void __launch_bounds__(kThreads, CTAS) k_q8_attn_few(const __grid_constant__ AttnArgs a)
 {
-    const long long unit = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    const int t = (int)(unit / a.n_q_heads), g = (int)(unit - (long long)t * a.n_q_heads);
-    if (t >= a.b.n_tokens) return;
-    q8::Entry e = {0, 0, 0, 0};
-    for (int i = 0; i < a.b.n_seqs; i++) {
-        const q8::Entry m = q8::entry(a.b, i);
-        if (m.n > 0 && t >= m.q0 && t < m.q0 + m.n) { e = m; break; }
+    constexpr int KS = HD / 16;               // k-steps of the scores, 32-bit code words of a K row in a lane
+    constexpr int VW = HD / 32;               // code words of a V row in a lane
+    constexpr bool kQInRegs = NT * KS <= 8;
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    FewSmem<HD, NT> &sm = *reinterpret_cast<FewSmem<HD, NT> *>(smem_raw);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
+    const int H = a.l.heads, G = a.group;
+
+    // ---- this CTA's run of tiles: sum over all entries, then the entry it begins in
+    unsigned total = 0;
+    for (int base = 0; base < a.b.n_seqs; base += kThreads) {
+        unsigned t = 0;
+        if (base + tid < a.b.n_seqs) t = unit_of(a, entry(a.b, base + tid)).tiles * H;
+#pragma unroll
+        for (int d = 16; d; d >>= 1) t += __shfl_xor_sync(0xffffffffu, t, d);
+        if (lane == 0) sm.scan[warp] = t;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kWarps; i++) total += sm.scan[i];
+        __syncthreads();
     }
-    if (e.n == 0) return;
-    const int pos = e.kv_len - e.n + t - e.q0;
-    const int end = a.causal ? pos + 1 : e.kv_len;
-    const int begin = a.window > 0 && pos - a.window + 1 > 0 ? pos - a.window + 1 : 0;
-    const long long slot = (long long)e.seq * a.l.heads + g / a.group;
-    const uint8_t *k = a.l.k + slot * a.l.max_seq * HD, *v = a.l.v + slot * a.l.max_seq * HD;
-    const float *ks = a.l.k_scale + slot * (a.l.max_seq >> a.l.block_log2);
-    const float *vs = a.l.v_scale + slot * (a.l.max_seq >> a.l.block_log2);
-    const T *q = static_cast<const T *>(a.q) + t * a.q_stride + g * HD;
-    float qr[HD / 32], acc[HD / 32], m = -INFINITY, sum = 0.0f;
+    const Runs runs = runs_of(total, gridDim.x);
+    if (blockIdx.x >= runs.n) return;
+    unsigned t = run_begin(runs, blockIdx.x);
+    const unsigned t_begin = t, t_end = run_begin(runs, blockIdx.x + 1);
+    unsigned before = 0;
+    for (int base = 0; base < a.b.n_seqs; base += kThreads) {
+        unsigned n = 0;
+        if (base + tid < a.b.n_seqs) n = unit_of(a, entry(a.b, base + tid)).tiles * H;
+        unsigned upto = n;
 #pragma unroll
-    for (int i = 0; i < HD / 32; i++) {
-        qr[i] = sp_load_as_float(q, lane + 32 * i) * a.scale;
-        acc[i] = 0.0f;
+        for (int d = 1; d < 32; d <<= 1) {
+            const unsigned o = __shfl_up_sync(0xffffffffu, upto, d);
+            if (lane >= d) upto += o;
+        }
+        if (lane == 31) sm.scan[warp] = upto;
+        __syncthreads();
+        unsigned sum = 0;
+#pragma unroll
+        for (int i = 0; i < kWarps; i++) {
+            if (i < warp) upto += sm.scan[i];
+            sum += sm.scan[i];
+        }
+        upto += before;
+        if (t >= upto - n && t < upto) {
+            sm.found[0] = base + tid;
+            sm.found[1] = upto - n;
+        }
+        before += sum;
+        __syncthreads();
+        if (t < before) break;
     }
-    for (int j = begin; j < end; j++) {
-        float s = 0.0f;
+    int ei = sm.found[0];
+    unsigned entry_t = sm.found[1];           // the entry's first tile
+    Entry e = entry(a.b, ei);
+    Unit0 u = unit_of(a, e);
+
+    while (t < t_end) {
+        while (t >= entry_t + u.tiles * H) {  // on to the next entry that has tiles
+            entry_t += u.tiles * H;
+            e = entry(a.b, ++ei);
+            u = unit_of(a, e);
+        }
+        const int head = (t - entry_t) / u.tiles;
+        const unsigned unit_t = entry_t + head * u.tiles;
+        const int k0 = t - unit_t, k1 = min((unsigned)u.tiles, t_end - unit_t);
+        const int rows = e.n * G, first = e.kv_len - e.n;
+        const long long slot = (long long)e.seq * H + head;
+        const uint8_t *kp = a.l.k + slot * a.l.max_seq * HD, *vp = a.l.v + slot * a.l.max_seq * HD;
+        const float *ksp = a.l.k_scale + slot * (a.l.max_seq >> a.l.block_log2);
+        const float *vsp = a.l.v_scale + slot * (a.l.max_seq >> a.l.block_log2);
+
+        uint32_t kw[2][KS], vw[4][VW];
+        float ks = 0.0f, vs = 1.0f;
+        auto load_k = [&](int j0) {
 #pragma unroll
-        for (int i = 0; i < HD / 32; i++) s += qr[i] * q8::decode1<FMT>(k[(long long)j * HD + lane + 32 * i]);
+            for (int r = 0; r < 2; r++)
 #pragma unroll
-        for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-        s *= ks[j >> a.l.block_log2];
-        const float top = fmaxf(m, s), fix = expf(m - top), p = expf(s - top);
-        m = top;
-        sum = sum * fix + p;
-        const float w = p * vs[j >> a.l.block_log2];
+                for (int j = 0; j < KS / 4; j++) {
+                    const uint4 w = ldg16(kp + (long long)(j0 + g + 8 * r) * HD + 64 * j + 16 * c);
+                    kw[r][4 * j] = w.x; kw[r][4 * j + 1] = w.y; kw[r][4 * j + 2] = w.z; kw[r][4 * j + 3] = w.w;
+                }
+            ks = ksp[j0 >> a.l.block_log2];
+        };
+        auto load_v = [&](int j0) {
 #pragma unroll
-        for (int i = 0; i < HD / 32; i++)
-            acc[i] = acc[i] * fix + w * q8::decode1<FMT>(v[(long long)j * HD + lane + 32 * i]);
+            for (int r = 0; r < 4; r++) {
+                const uint8_t *p = vp + (long long)(j0 + 2 * c + (r & 1) + 8 * (r >> 1)) * HD;
+                if constexpr (HD == 64) {
+                    const uint2 w = ldg8(p + 8 * g);
+                    vw[r][0] = w.x; vw[r][1] = w.y;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < HD / 128; i++) {
+                        const uint4 w = ldg16(p + 128 * i + 16 * g);
+                        vw[r][4 * i] = w.x; vw[r][4 * i + 1] = w.y; vw[r][4 * i + 2] = w.z; vw[r][4 * i + 3] = w.w;
+                    }
+                }
+            }
+            vs = vsp[j0 >> a.l.block_log2];
+        };
+        // dimension of code word i of a V row
+        auto dim_of = [&](int i) { return HD == 64 ? 8 * g + 4 * i : 128 * (i / 4) + 16 * g + 4 * (i % 4); };
+
+        int j0 = u.start + k0 * kTile + 16 * warp;
+        const int j_stop = min(u.end, u.start + k1 * kTile);
+        if (j0 < j_stop) { load_k(j0); load_v(j0); }
+
+        // ---- queries: scaled to fp16, in fragment order
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            const int row = 8 * n + warp;
+            constexpr int E = HD / 32;
+            float x[E], top = 0.0f;
+            if (row < rows) {
+                const T *q = static_cast<const T *>(a.q) + (long long)(e.q0 + row / G) * a.q_stride + (head * G + row % G) * HD;
+#pragma unroll
+                for (int i = 0; i < E; i++) {
+                    x[i] = sp_load_as_float(q, lane + 32 * i);
+                    top = fmaxf(top, fabsf(x[i]));
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < E; i++) x[i] = 0.0f;
+            }
+#pragma unroll
+            for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+            float down, up;
+            row_scale(top, down, up);
+            if (lane == 0) sm.up[row] = up;
+#pragma unroll
+            for (int i = 0; i < E; i++) {
+                const int d = lane + 32 * i, s = d / 64 * 4 + d % 16 / 4, p = d % 4;
+                // word order (0, 2), (1, 3): unpack4's pairs
+                reinterpret_cast<__half *>(&sm.q[n][s][4 * warp + d % 64 / 16])[(p >> 1) + 2 * (p & 1)] = __float2half_rn(x[i] * down);
+            }
+        }
+        __syncthreads();
+
+        uint2 qr[kQInRegs ? NT : 1][kQInRegs ? KS : 1];
+        if constexpr (kQInRegs) {
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int s = 0; s < KS; s++) qr[n][s] = sm.q[n][s][lane];
+        }
+        float mul[NT][2], m[NT][2], l[NT][2];
+        int hi[NT][2], lo[NT][2];
+        const int hi_min = a.causal ? first : e.kv_len - 1;
+        const int lo_max = a.window > 0 ? e.kv_len - a.window : 0;
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const int row = 8 * n + 2 * c + i, pos = first + row / G;
+                mul[n][i] = a.scale * kLog2e * sm.up[row] * (1.0f / Unit<FMT>::v);
+                hi[n][i] = a.causal ? pos : e.kv_len - 1;
+                lo[n][i] = a.window > 0 ? pos - a.window + 1 : 0;
+                m[n][i] = kNone;
+                l[n][i] = 0.0f;
+            }
+        float o[NT][2 * VW][4];
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int i = 0; i < 2 * VW; i++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) o[n][i][j] = 0.0f;
+
+        for (; j0 < j_stop; j0 += kTile) {
+            // ---- scores of 16 positions
+            float s[NT][4];
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) s[n][j] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < KS; i++) {
+                uint32_t f[4];
+                unpack4<FMT>(kw[0][i], f[0], f[2]);
+                unpack4<FMT>(kw[1][i], f[1], f[3]);
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    const uint2 b = kQInRegs ? qr[kQInRegs ? n : 0][kQInRegs ? i : 0] : sm.q[n][i][lane];
+                    mma(s[n], f, b.x, b.y);
+                }
+            }
+            const float k_scale = ks, v_scale = fmaxf(vs, kScaleMin);
+            const int next = j0 + kTile;
+            if (next < j_stop) load_k(next);
+
+            // ---- weights
+            const float lv = lg2(v_scale), iv = __frcp_rn(v_scale);
+            const bool all = j0 + 15 <= hi_min && j0 >= lo_max;     // nothing is masked
+            bool over = false;
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const float f = k_scale * mul[n][i];
+                    s[n][i] = fmaf(s[n][i], f, lv);
+                    s[n][2 + i] = fmaf(s[n][2 + i], f, lv);
+                    if (!all) {
+                        const int j = j0 + g;
+                        if (j > hi[n][i] || j < lo[n][i]) s[n][i] = -INFINITY;
+                        if (j + 8 > hi[n][i] || j + 8 < lo[n][i]) s[n][2 + i] = -INFINITY;
+                    }
+                    over |= fmaxf(s[n][i], s[n][2 + i]) > m[n][i] + 8.0f;
+                }
+            if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        float top = fmaxf(s[n][i], s[n][2 + i]);
+#pragma unroll
+                        for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                        top = fmaxf(top, m[n][i]);
+                        const float fix = ex2(m[n][i] - top);
+                        m[n][i] = top;
+                        l[n][i] *= fix;
+#pragma unroll
+                        for (int x = 0; x < 2 * VW; x++) {
+                            o[n][x][i] *= fix;
+                            o[n][x][2 + i] *= fix;
+                        }
+                    }
+            }
+            uint32_t p[NT][2];
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    s[n][i] = ex2(s[n][i] - m[n][i]);
+                    s[n][2 + i] = ex2(s[n][2 + i] - m[n][i]);
+                    l[n][i] = fmaf(s[n][i] + s[n][2 + i], iv, l[n][i]);
+                }
+#pragma unroll
+                for (int r = 0; r < 2; r++) {
+                    const __half2 h = __floats2half2_rn(s[n][2 * r], s[n][2 * r + 1]);
+                    p[n][r] = transpose8x8(*reinterpret_cast<const uint32_t *>(&h));
+                }
+            }
+            // ---- values
+#pragma unroll
+            for (int i = 0; i < VW; i++) {
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    uint32_t f[4];
+                    const unsigned pick = h ? 0x7632 : 0x5410;
+                    unpack4<FMT>(__byte_perm(vw[0][i], vw[1][i], pick), f[0], f[1]);
+                    unpack4<FMT>(__byte_perm(vw[2][i], vw[3][i], pick), f[2], f[3]);
+#pragma unroll
+                    for (int n = 0; n < NT; n++) mma(o[n][2 * i + h], f, p[n][0], p[n][1]);
+                }
+            }
+            if (next < j_stop) load_v(next);
+        }
+
+        // ---- the warps' results into one: rows lie in shared memory in the
+        // order (even rows, odd rows) of each 8, so a quarter warp's 16-byte
+        // stores fall on different banks
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) l[n][i] += __shfl_xor_sync(0xffffffffu, l[n][i], d);
+                if (g == 0) {
+                    sm.m[warp][8 * n + 2 * c + i] = m[n][i];
+                    sm.l[warp][8 * n + 2 * c + i] = l[n][i];
+                }
+            }
+        __syncthreads();
+        float fix[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                float top = kNone;
+#pragma unroll
+                for (int w = 0; w < kWarps; w++) top = fmaxf(top, sm.m[w][8 * n + 2 * c + i]);
+                fix[n][i] = ex2(m[n][i] - top);
+            }
+#pragma unroll
+        for (int half = 1; half >= 0; half--) {
+            if ((warp >> 2) == half) {
+                float(*dst)[HD + 4] = sm.o[warp & 3];
+#pragma unroll
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int x = 0; x < VW; x++)
+#pragma unroll
+                        for (int i = 0; i < 2; i++) {
+                            float4 *at = reinterpret_cast<float4 *>(&dst[8 * n + c + 4 * i][dim_of(x)]);
+                            float4 v = make_float4(o[n][2 * x][i] * fix[n][i], o[n][2 * x][2 + i] * fix[n][i],
+                                                   o[n][2 * x + 1][i] * fix[n][i], o[n][2 * x + 1][2 + i] * fix[n][i]);
+                            if (half == 0) {
+                                const float4 w = *at;
+                                v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
+                            }
+                            *at = v;
+                        }
+            }
+            __syncthreads();
+        }
+
+        // ---- the unit's result, or this run's part of it
+        const bool whole = k0 == 0 && k1 == u.tiles;
+        const unsigned run0 = run_of_tile(runs, unit_t), run1 = run_of_tile(runs, unit_t + u.tiles - 1);
+        constexpr int kSlot = 8 * NT * (HD + 2);
+        constexpr float kOut = 1.0f / Unit<FMT>::v;
+        auto finish = [&](int row, int d, float4 v, float top, float sum) {
+            const float inv = sum > 0.0f ? kOut / sum : 0.0f;
+            T w[4] = {T(v.x * inv), T(v.y * inv), T(v.z * inv), T(v.w * inv)};
+            const long long tok = e.q0 + row / G;
+            const int qh = head * G + row % G;
+            *reinterpret_cast<uint2 *>(static_cast<T *>(a.out) + tok * a.out_stride + qh * HD + d) = *reinterpret_cast<uint2 *>(w);
+            if (a.lse && d == 0) a.lse[tok * a.n_q_heads + qh] = sum > 0.0f ? kLn2 * (top + lg2(sum)) : -INFINITY;
+        };
+        // slots: a run has at most one unit that began before it and one that goes on after it
+        float *part = a.partials + (2 * blockIdx.x + (unit_t >= t_begin)) * kSlot;
+        for (int i = tid; i < rows * (HD / 4); i += kThreads) {
+            const int row = i / (HD / 4), d = i % (HD / 4) * 4, at = (row & ~7) + (row & 7) / 2 + 4 * (row & 1);
+            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                const float4 x = *reinterpret_cast<const float4 *>(&sm.o[w][at][d]);
+                v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
+            }
+            float top = kNone, sum = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kWarps; w++) top = fmaxf(top, sm.m[w][row]);
+#pragma unroll
+            for (int w = 0; w < kWarps; w++) sum += sm.l[w][row] * ex2(sm.m[w][row] - top);
+            if (whole) {
+                finish(row, d, v, top, sum);
+            } else {
+                __stcg(reinterpret_cast<float4 *>(part + row * HD + d), v);
+                if (d == 0) __stcg(reinterpret_cast<float2 *>(part + 8 * NT * HD + 2 * row), make_float2(top, sum));
+            }
+        }
+        if (!whole) {
+            __threadfence();
+            __syncthreads();
+            if (tid == 0) sm.last = atomicAdd(a.counters + run0, 1u) == run1 - run0;
+            __syncthreads();
+            if (sm.last) {
+                __threadfence();
+                if (tid == 0) a.counters[run0] = 0;
+                auto slot_of = [&](unsigned r) { return a.partials + (2 * r + (run_begin(runs, r) <= unit_t)) * kSlot; };
+                for (int i = tid; i < rows * (HD / 4); i += kThreads) {
+                    const int row = i / (HD / 4), d = i % (HD / 4) * 4;
+                    float top = kNone, sum = 0.0f;
+                    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    for (unsigned r = run0; r <= run1; r += 8) {
+                        float2 ml[8];
+                        float4 x[8];
+                        float up = top;
+#pragma unroll
+                        for (int k = 0; k < 8; k++) {
+                            ml[k] = make_float2(kNone, 0.0f);
+                            x[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                            if (r + k <= run1) {
+                                const float *q = slot_of(r + k);
+                                ml[k] = __ldcg(reinterpret_cast<const float2 *>(q + 8 * NT * HD + 2 * row));
+                                x[k] = __ldcg(reinterpret_cast<const float4 *>(q + row * HD + d));
+                            }
+                        }
+#pragma unroll
+                        for (int k = 0; k < 8; k++) up = fmaxf(up, ml[k].x);
+                        const float old = ex2(top - up);
+                        sum *= old;
+                        v.x *= old; v.y *= old; v.z *= old; v.w *= old;
+#pragma unroll
+                        for (int k = 0; k < 8; k++) {
+                            const float f = ex2(ml[k].x - up);
+                            sum = fmaf(ml[k].y, f, sum);
+                            v.x = fmaf(x[k].x, f, v.x);
+                            v.y = fmaf(x[k].y, f, v.y);
+                            v.z = fmaf(x[k].z, f, v.z);
+                            v.w = fmaf(x[k].w, f, v.w);
+                        }
+                        top = up;
+                    }
+                    finish(row, d, v, top, sum);
+                }
+            }
+        }
+        t = unit_t + k1;
+        __syncthreads();                       // shared memory is free for the next unit
     }
-    T *out = static_cast<T *>(a.out) + t * a.out_stride + g * HD;
-    const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
-#pragma unroll
-    for (int i = 0; i < HD / 32; i++) out[lane + 32 * i] = T(acc[i] * inv);
-    if (a.lse && lane == 0) a.lse[(long long)t * a.n_q_heads + g] = m + logf(sum);
+}
+
+template <typename T, int FMT, int HD, int NT>
+int launch_few(const AttnArgs &a, int sms, unsigned tiles, cudaStream_t s)
+{
+    // CTAs on an SM: what the registers of 256 threads allow without spilling
+    constexpr int CTAS = NT * HD <= 64 ? 3 : NT * HD <= 128 ? 2 : 1;
+    auto kernel = k_q8_attn_few<T, FMT, HD, NT, CTAS>;
+    constexpr int smem = sizeof(FewSmem<HD, NT>);
+    static std::atomic<unsigned long long> ready{0};      // devices whose attribute is set
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (smem > 48 * 1024 && !(ready.load(std::memory_order_acquire) >> (dev & 63) & 1)) {
+        const int rc = sp_check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
+                                     "q8_attn shared memory");
+        if (rc) return rc;
+        if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_release);
+    }
+    unsigned grid = (unsigned)(sms * CTAS);
+    if (grid > (unsigned)kMaxCtas) grid = kMaxCtas;
+    if (grid > tiles) grid = tiles;
+    kernel<<<grid, kThreads, smem, s>>>(a);
+    return sp_check_cuda(cudaGetLastError(), "q8_attn launch");
 }
 
 template <typename T, int FMT>
-void launch_rows(const AttnArgs &a, int hd, unsigned grid, cudaStream_t s)
+int launch_few_of(const AttnArgs &a, int hd, int nt, int sms, unsigned tiles, cudaStream_t s)
 {
-    if (hd == 64) k_q8_attn_rows<T, FMT, 64><<<grid, 128, 0, s>>>(a);
-    else if (hd == 128) k_q8_attn_rows<T, FMT, 128><<<grid, 128, 0, s>>>(a);
-    else k_q8_attn_rows<T, FMT, 256><<<grid, 128, 0, s>>>(a);
+    if (hd == 64) return nt == 1 ? launch_few<T, FMT, 64, 1>(a, sms, tiles, s) : nt == 2 ? launch_few<T, FMT, 64, 2>(a, sms, tiles, s)
+                                                                                          : launch_few<T, FMT, 64, 4>(a, sms, tiles, s);
+    if (hd == 128) return nt == 1 ? launch_few<T, FMT, 128, 1>(a, sms, tiles, s) : nt == 2 ? launch_few<T, FMT, 128, 2>(a, sms, tiles, s)
+                                                                                            : launch_few<T, FMT, 128, 4>(a, sms, tiles, s);
+    return nt == 1 ? launch_few<T, FMT, 256, 1>(a, sms, tiles, s) : launch_few<T, FMT, 256, 2>(a, sms, tiles, s);
 }
 
 }  // namespace
+
+namespace q8 {
+// Counters, then the partial results of the larger grid: two slots for each
+// CTA of up to 32 rows at up to three CTAs an SM, or of 256 rows at one.
+size_t attn_workspace_bytes(int sm_count, int head_dim)
+{
+    const size_t few = (size_t)2 * 3 * sm_count * 32 * (head_dim + 2) * sizeof(float);
+    const size_t many = (size_t)2 * sm_count * 256 * (head_dim + 2) * sizeof(float);
+    return kMaxCtas * sizeof(unsigned) + (few > many ? few : many);
+}
+}  // namespace q8
 
 extern "C" int sp_cuda_q8_attn(const sp_cuda_q8_cache_t *qc, int layer, const sp_cuda_q8_batch_t *batch, const void *d_q,
                                long long q_stride, int n_q_heads, int dtype, float logit_scale, int causal, int window,
@@ -110,18 +546,32 @@ extern "C" int sp_cuda_q8_attn(const sp_cuda_q8_cache_t *qc, int layer, const sp
     if (!d_q || !d_out) return sp_set_error(SP_ERR_ARG, "q8_attn: NULL argument");
     if (((uintptr_t)d_q | (uintptr_t)d_out | (uintptr_t)(q_stride * 2) | (uintptr_t)(out_stride * 2)) % 16 || (uintptr_t)d_lse % 4)
         return sp_set_error(SP_ERR_ARG, "q8_attn: pointers and strides must be multiples of 16 bytes");
+    const int G = n_q_heads / H;
     AttnArgs a = {q8::layer_of(qc, layer), q8::batch_of(qc, batch), d_q, d_out, d_lse, q_stride, out_stride,
-                  n_q_heads, n_q_heads / H, logit_scale, causal, window};
-    const long long units = (long long)batch->n_tokens * n_q_heads;
-    if (units > 0x7fffffff) return sp_set_error(SP_ERR_ARG, "q8_attn: %lld rows in one call", units);
-    const unsigned grid = (unsigned)((units + 3) / 4);
+                  n_q_heads, G, logit_scale, causal, window, 0, (unsigned int *)qc->d_attn_ws,
+                  (float *)qc->d_attn_ws + kMaxCtas};
+    const long long tiles = (long long)batch->n_seqs * H * (batch->max_kv / kTile + 2);
+    const long long rows = (long long)batch->max_new * G;
+    if (tiles > 0x7fffffff) return sp_set_error(SP_ERR_ARG, "q8_attn: %lld tiles in one call", tiles);
+    // The few-row kernel takes entries of up to 8, 16 or 32 rows (32 only where
+    // the accumulators of head_dim 256 do not fill the registers).  Where the
+    // batch has longer entries it takes those of one token or so, and the
+    // many-row kernel the others.
+    const int most = hd == 256 ? 16 : 32;
+    const long long take = rows <= most ? rows : G;
+    const int nt = take <= 8 ? 1 : take <= 16 ? 2 : take <= most ? 4 : 0;
+    a.few_rows = 8 * nt;
     cudaStream_t s = (cudaStream_t)stream;
-    if (dtype == SP_DTYPE_F16) {
-        if (qc->format == SP_Q8_INT8) launch_rows<__half, SP_Q8_INT8>(a, hd, grid, s);
-        else launch_rows<__half, SP_Q8_E4M3>(a, hd, grid, s);
-    } else {
-        if (qc->format == SP_Q8_INT8) launch_rows<__nv_bfloat16, SP_Q8_INT8>(a, hd, grid, s);
-        else launch_rows<__nv_bfloat16, SP_Q8_E4M3>(a, hd, grid, s);
+    const bool i8 = qc->format == SP_Q8_INT8;
+    if (nt) {
+        if (dtype == SP_DTYPE_F16)
+            rc = i8 ? launch_few_of<__half, SP_Q8_INT8>(a, hd, nt, qc->sm_count, (unsigned)tiles, s)
+                    : launch_few_of<__half, SP_Q8_E4M3>(a, hd, nt, qc->sm_count, (unsigned)tiles, s);
+        else
+            rc = i8 ? launch_few_of<__nv_bfloat16, SP_Q8_INT8>(a, hd, nt, qc->sm_count, (unsigned)tiles, s)
+                    : launch_few_of<__nv_bfloat16, SP_Q8_E4M3>(a, hd, nt, qc->sm_count, (unsigned)tiles, s);
+        if (rc) return rc;
     }
-    return sp_check_cuda(cudaGetLastError(), "q8_attn launch");
+    if (rows > a.few_rows) rc = q8::launch_many(a, qc->format, dtype, hd, qc->sm_count, s);
+    return rc;
 }

@@ -1,0 +1,108 @@
+// sp_q8_attn.cuh — arguments, work split and workspace shared by the
+// attention kernels over the 8-bit cache.
+#pragma once
+
+#include "sp_q8.cuh"
+
+namespace q8 {
+
+struct AttnArgs {
+    Layer l;
+    Batch b;
+    const void *q;
+    void *out;
+    float *lse;                      // NULL: not wanted
+    long long q_stride, out_stride;  // elements between tokens
+    int n_q_heads, group;
+    float scale;                     // logit scale
+    int causal, window;
+    int few_rows;                    // entries of up to so many rows (new tokens x group) are the
+                                     // few-row kernel's, the others the many-row kernel's
+    unsigned int *counters;          // [kMaxCtas], zero between calls
+    float *partials;
+};
+
+constexpr int kMaxCtas = 1024;       // most CTAs of an attention grid
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kNone = -3.402823466e38f;    // running maximum of a row that has seen nothing
+
+// --- work split -------------------------------------------------------
+// A call's tiles of positions, laid end to end over its units of work, are
+// cut into equal runs, one for each CTA, whatever the lengths; a unit that
+// falls into several runs leaves a partial result (maximum, sum, weighted
+// values) for each, and the CTA that finishes last joins them in run order,
+// so results do not depend on the order of arrival.
+struct Runs {
+    unsigned total, n, q, r;         // tiles, CTAs with work, tiles of a run (the first r have one more)
+};
+
+__device__ __forceinline__ Runs runs_of(unsigned total, unsigned grid)
+{
+    Runs s;
+    s.total = total;
+    s.n = min(total, grid);
+    s.q = s.n ? total / s.n : 0;
+    s.r = s.n ? total - s.q * s.n : 0;
+    return s;
+}
+__device__ __forceinline__ unsigned run_begin(const Runs &s, unsigned i) { return i * s.q + min(i, s.r); }
+__device__ __forceinline__ unsigned run_of_tile(const Runs &s, unsigned t)
+{
+    const unsigned cut = s.r * (s.q + 1);
+    return t < cut ? t / (s.q + 1) : s.r + (t - cut) / s.q;
+}
+
+// --- small things -----------------------------------------------------
+__device__ __forceinline__ float ex2(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float lg2(float x)
+{
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Four codes (bytes 0..3 of x) as fp16 pairs, lo = (byte 0, byte 2) and
+// hi = (byte 1, byte 3), each the code's value times kUnit<FMT>, exactly and
+// finite for every byte.
+//   int8: q + 128 placed in the low mantissa of 1024, then 1152 taken off.
+//   e4m3: sign, exponent and mantissa moved into an fp16's fields; the
+//   exponents' biases differ by 8, which the subnormals follow.
+template <int FMT> struct Unit;
+template <> struct Unit<SP_Q8_INT8> { static constexpr float v = 1.0f; };
+template <> struct Unit<SP_Q8_E4M3> { static constexpr float v = 0x1p-8f; };
+
+template <int FMT>
+__device__ __forceinline__ void unpack4(uint32_t x, uint32_t &lo, uint32_t &hi)
+{
+    if constexpr (FMT == SP_Q8_INT8) {
+        x ^= 0x80808080u;
+        const uint32_t a = __byte_perm(x, 0x64646464u, 0x4240), b = __byte_perm(x, 0x64646464u, 0x4341);
+        const __half2 c = __half2half2(__ushort_as_half(0x6480));       // 1152
+        const __half2 u = __hsub2(*reinterpret_cast<const __half2 *>(&a), c);
+        const __half2 v = __hsub2(*reinterpret_cast<const __half2 *>(&b), c);
+        lo = *reinterpret_cast<const uint32_t *>(&u);
+        hi = *reinterpret_cast<const uint32_t *>(&v);
+    } else {
+        lo = ((x << 7) & 0x3f803f80u) | ((x << 8) & 0x80008000u);
+        hi = ((x >> 1) & 0x3f803f80u) | (x & 0x80008000u);
+    }
+}
+
+// 2^-e and 2^e for a row of queries whose largest magnitude is top, e its
+// exponent: scaled rows fit fp16 whatever their type's range.
+__device__ __forceinline__ void row_scale(float top, float &down, float &up)
+{
+    const unsigned E = (__float_as_uint(top) >> 23) & 0xff;
+    const unsigned F = top > 0.0f && E < 255 ? min(max(E, 1u), 253u) : 127u;
+    down = __uint_as_float((254u - F) << 23);
+    up = __uint_as_float(F << 23);
+}
+
+int launch_many(const AttnArgs &a, int format, int dtype, int hd, int sms, cudaStream_t s);   // sp_q8_attn_many.cu
+
+}  // namespace q8
