@@ -103,6 +103,7 @@ __device__ __forceinline__ void row_scale(float top, float &down, float &up)
     up = __uint_as_float(F << 23);
 }
 
-int launch_many(const AttnArgs &a, int format, int dtype, int hd, int sms, cudaStream_t s);   // sp_q8_attn_many.cu
+size_t split_bytes(int sm_count);                                    // sp_q8_attn_many.cu
+int launch_many(const AttnArgs &a, int format, int dtype, int hd, int sms, cudaStream_t s);
 
 }  // namespace q8

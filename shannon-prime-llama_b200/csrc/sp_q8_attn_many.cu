@@ -1,87 +1,709 @@
 // sp_q8_attn_many.cu — attention over the 8-bit cache for many rows (prompts
-// and chunks of prompts).
+// and chunks of prompts) on the 5th-generation tensor cores.
+//
+// Rows of a unit of work are its tokens times the query heads that share the
+// KV head, 256 at a time (128 at head_dim 256), against tiles of 128 (64)
+// positions:
+//     S = Q K'      both from shared memory, into tensor memory
+//     P = 2^(S f + log2 vs - m), by the rows' own threads, back into the
+//         columns of S as fp16 (the softmax of sp_q8_attn.cu)
+//     O += P V      P from tensor memory, V from shared memory
+// Codes become fp16 once for all 256 rows: eight warps load them, unpack them
+// in registers and store them in the core-matrix layout (8 rows of 16 bytes)
+// that serves K as the K-major and V as the MN-major operand.  One thread
+// issues the products; while a softmax warpgroup works on its 128 rows, the
+// tensor cores work on the other 128.
 #include "sp_q8_attn.cuh"
+#include "sp_bulk.cuh"
+
+#include <atomic>
 
 namespace {
 
 using namespace q8;
 
-// One warp for each (token, query head): one pass over the positions that the
-// token sees with a running maximum and sum, a lane holding every 32nd
-// element of the head.
-template <typename T, int FMT, int HD>
-__global__ void __launch_bounds__(128) k_q8_attn_rows(const __grid_constant__ AttnArgs a)
+template <int HD>
+struct Shape {
+    static constexpr int NQ = HD == 256 ? 1 : 2;       // 128-row tiles of queries
+    static constexpr int BN = HD == 256 ? 64 : 128;    // positions of a tile
+    static constexpr int ROWS = 128 * NQ;
+    static constexpr int SoftWarps = 4 * NQ, ConvWarps = 8;
+    static constexpr int Threads = 32 * (SoftWarps + ConvWarps + 1);
+    static constexpr int ColO = 256;                   // S (and P) at 128 i or 64 (k & 1), O at 256 + HD i
+    static constexpr int StageB = BN * HD * 2, QB = 128 * HD * 2;
+    static constexpr int SlotFloats = ROWS * (HD + 2);
+};
+
+template <int HD>
+struct ManySmem {
+    unsigned char q[Shape<HD>::NQ][Shape<HD>::QB];
+    unsigned char k[2][Shape<HD>::StageB], v[2][Shape<HD>::StageB];
+    unsigned long long q_full[2], k_full[2], k_free[2], v_full[2], v_free[2], s_full[2], p_full[2], pv_done[2], end;
+    unsigned scan[32];
+    unsigned tiles[256];                               // of one head of each entry of a chunk, then their prefix
+    int found;
+    unsigned found_t;
+    uint32_t tmem;
+    int abort;
+};
+
+// What the join kernel needs of a unit that falls into several runs; kept by
+// the run in which the unit begins.
+struct Split {
+    int valid, q0, row0, rows, head;
+    unsigned unit_t, run0, run1;
+};
+
+// --- tensor core and tensor memory --------------------------------------
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+#define Q8_R8(b) "=r"(v[b]), "=r"(v[b + 1]), "=r"(v[b + 2]), "=r"(v[b + 3]), "=r"(v[b + 4]), "=r"(v[b + 5]), "=r"(v[b + 6]), "=r"(v[b + 7])
+__device__ __forceinline__ void tmem_ld32(uint32_t at, uint32_t (&v)[32])
 {
-    const long long unit = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    const int t = (int)(unit / a.n_q_heads), g = (int)(unit - (long long)t * a.n_q_heads);
-    if (t >= a.b.n_tokens) return;
-    Entry e = {0, 0, 0, 0};
-    for (int i = 0; i < a.b.n_seqs; i++) {
-        const Entry m = entry(a.b, i);
-        if (m.n > 0 && t >= m.q0 && t < m.q0 + m.n) { e = m; break; }
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
+                 "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : Q8_R8(0), Q8_R8(8), Q8_R8(16), Q8_R8(24) : "r"(at));
+}
+#undef Q8_R8
+#define Q8_R8(b) "r"(v[b]), "r"(v[b + 1]), "r"(v[b + 2]), "r"(v[b + 3]), "r"(v[b + 4]), "r"(v[b + 5]), "r"(v[b + 6]), "r"(v[b + 7])
+__device__ __forceinline__ void tmem_st32(uint32_t at, const uint32_t (&v)[32])
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
+                 "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
+                 ::"r"(at), Q8_R8(0), Q8_R8(8), Q8_R8(16), Q8_R8(24) : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t (&v)[16])
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+                 ::"r"(at), Q8_R8(0), Q8_R8(8) : "memory");
+}
+#undef Q8_R8
+
+// Shared-memory operand without swizzle, in core matrices of 8 rows of 16
+// bytes: byte offsets between core matrices along and across the leading
+// direction (K-major: lbo along K, sbo along M or N; MN-major: lbo along K,
+// sbo along M or N too).
+__device__ __forceinline__ uint64_t operand(uint32_t addr, uint32_t lbo, uint32_t sbo)
+{
+    return (uint64_t)((addr & 0x3FFFFu) >> 4) | (uint64_t)((lbo >> 4) & 0x3FFFu) << 16 |
+           (uint64_t)((sbo >> 4) & 0x3FFFu) << 32 | (uint64_t)1 << 46;
+}
+
+// fp16 x fp16 -> fp32, M = 128
+constexpr uint32_t instr(int n, bool b_mn)
+{
+    return (1u << 4) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t i, uint32_t add)
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %3, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %4, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(add), "r"(i)
+                 : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t i, uint32_t add)
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %3, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %4, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(add), "r"(i)
+                 : "memory");
+}
+__device__ __forceinline__ void commit(uint32_t bar)
+{
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void arrive(uint32_t bar)
+{
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+// Waits for a phase; false once any wait of this CTA has run out (2 s).
+__device__ __noinline__ bool wait_slow(uint32_t bar, uint32_t parity, int *abort, unsigned int *status)
+{
+    const unsigned long long t0 = spb::global_ns();
+    for (;;) {
+        for (int i = 0; i < 64; i++)
+            if (spb::mbar_try_wait(bar, parity)) return true;
+        if (*(volatile int *)abort) return false;
+        if (spb::global_ns() - t0 > spb::kWaitLimitNs) break;
     }
-    if ((long long)e.n * a.group <= a.few_rows) return;
-    const int pos = e.kv_len - e.n + t - e.q0;
-    const int end = a.causal ? pos + 1 : e.kv_len;
-    const int begin = a.window > 0 && pos - a.window + 1 > 0 ? pos - a.window + 1 : 0;
-    const long long slot = (long long)e.seq * a.l.heads + g / a.group;
-    const uint8_t *k = a.l.k + slot * a.l.max_seq * HD, *v = a.l.v + slot * a.l.max_seq * HD;
-    const float *ks = a.l.k_scale + slot * (a.l.max_seq >> a.l.block_log2);
-    const float *vs = a.l.v_scale + slot * (a.l.max_seq >> a.l.block_log2);
-    const T *q = static_cast<const T *>(a.q) + t * a.q_stride + g * HD;
-    float qr[HD / 32], acc[HD / 32], m = -INFINITY, sum = 0.0f;
-#pragma unroll
-    for (int i = 0; i < HD / 32; i++) {
-        qr[i] = sp_load_as_float(q, lane + 32 * i) * a.scale;
-        acc[i] = 0.0f;
+    *(volatile int *)abort = 1;
+    if (status) atomicOr(status, 2u);
+    return false;
+}
+
+// --- units: (entry, KV head, tile of rows) ------------------------------
+struct Rows {
+    int row0, rows, start, tiles;
+};
+
+template <int HD>
+__device__ __forceinline__ int row_tiles(const AttnArgs &a, const Entry &e)
+{
+    const long long r = (long long)e.n * a.group;
+    return r <= a.few_rows ? 0 : (int)((r + Shape<HD>::ROWS - 1) / Shape<HD>::ROWS);
+}
+
+template <int HD>
+__device__ __forceinline__ Rows rows_of(const AttnArgs &a, const Entry &e, int qt)
+{
+    constexpr int BN = Shape<HD>::BN;
+    Rows r;
+    r.row0 = qt * Shape<HD>::ROWS;
+    r.rows = min(Shape<HD>::ROWS, e.n * a.group - r.row0);
+    const int first = e.kv_len - e.n;
+    const int lo = first + r.row0 / a.group, hi = first + (r.row0 + r.rows - 1) / a.group;
+    const int end = a.causal ? hi + 1 : e.kv_len;
+    r.start = a.window > 0 && lo - a.window + 1 > 0 ? (lo - a.window + 1) / BN * BN : 0;
+    r.tiles = max(1, (end - r.start + BN - 1) / BN);
+    return r;
+}
+
+// Walks the units of a run: every role goes through the same ones.
+template <int HD>
+struct Walk {
+    Entry e;
+    int ei, qt, n_qt, head;
+    unsigned t, t_end, unit_t;      // next tile, end of the run, first tile of the unit
+    Rows r;
+    __device__ __forceinline__ bool more() const { return t < t_end; }
+    __device__ __forceinline__ int k0() const { return t - unit_t; }
+    __device__ __forceinline__ int k1() const { return min((unsigned)r.tiles, t_end - unit_t); }
+    __device__ __forceinline__ void next(const AttnArgs &a)
+    {
+        t = unit_t + k1();
+        if (t >= t_end) return;
+        unit_t += r.tiles;
+        if (++qt == n_qt) {
+            qt = 0;
+            if (++head == a.l.heads) {
+                head = 0;
+                do {
+                    e = entry(a.b, ++ei);
+                    n_qt = row_tiles<HD>(a, e);
+                } while (n_qt == 0);
+            }
+        }
+        r = rows_of<HD>(a, e, qt);
     }
-    for (int j = begin; j < end; j++) {
-        float s = 0.0f;
+};
+
+template <typename T, int FMT, int HD>
+__global__ void __launch_bounds__(Shape<HD>::Threads, 1) k_q8_attn_many(const __grid_constant__ AttnArgs a)
+{
+    using S = Shape<HD>;
+    constexpr int NQ = S::NQ, BN = S::BN;
+    extern __shared__ __align__(128) unsigned char smem_raw[];
+    ManySmem<HD> &sm = *reinterpret_cast<ManySmem<HD> *>(smem_raw);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    constexpr int kWarps = S::Threads / 32;
+    Split *splits = reinterpret_cast<Split *>(a.counters + kMaxCtas) + blockIdx.x;
+    if (tid == 0) splits->valid = 0;
+
+    // ---- this CTA's run: tiles of one head of each entry (a warp for an entry, a lane for
+    // a tile of rows), their sum, and the entry in which the run begins
+    Runs runs;
+    unsigned before = 0;
+    for (int pass = 0; pass < 2; pass++) {
+        before = 0;
+        for (int base = 0; base < a.b.n_seqs; base += 256) {
+            const int n = min(256, a.b.n_seqs - base);
+            for (int i = warp; i < n; i += kWarps) {
+                const Entry e = entry(a.b, base + i);
+                const int nq = row_tiles<HD>(a, e);
+                unsigned sum = 0;
+                for (int q = lane; q < nq; q += 32) sum += rows_of<HD>(a, e, q).tiles;
 #pragma unroll
-        for (int i = 0; i < HD / 32; i++) s += qr[i] * decode1<FMT>(k[(long long)j * HD + lane + 32 * i]);
+                for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+                if (lane == 0) sm.tiles[i] = sum * a.l.heads;
+            }
+            __syncthreads();
+            if (warp == 0) {
+                for (int i = 0; i < n; i += 32) {
+                    const unsigned x = i + lane < n ? sm.tiles[i + lane] : 0;
+                    unsigned upto = x;
 #pragma unroll
-        for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-        s *= ks[j >> a.l.block_log2];
-        const float top = fmaxf(m, s), fix = expf(m - top), p = expf(s - top);
-        m = top;
-        sum = sum * fix + p;
-        const float w = p * vs[j >> a.l.block_log2];
-#pragma unroll
-        for (int i = 0; i < HD / 32; i++)
-            acc[i] = acc[i] * fix + w * decode1<FMT>(v[(long long)j * HD + lane + 32 * i]);
+                    for (int d = 1; d < 32; d <<= 1) {
+                        const unsigned o = __shfl_up_sync(0xffffffffu, upto, d);
+                        if (lane >= d) upto += o;
+                    }
+                    if (pass) {
+                        const unsigned t = run_begin(runs, blockIdx.x);
+                        if (t >= before + upto - x && t < before + upto) {
+                            sm.found = base + i + lane;
+                            sm.found_t = before + upto - x;
+                        }
+                    }
+                    before += __shfl_sync(0xffffffffu, upto, 31);
+                }
+                if (lane == 0) sm.scan[0] = before;
+            }
+            __syncthreads();
+            before = sm.scan[0];
+            __syncthreads();
+        }
+        if (pass == 0) {
+            runs = runs_of(before, gridDim.x);
+            if (blockIdx.x >= runs.n) return;
+        }
     }
-    T *out = static_cast<T *>(a.out) + t * a.out_stride + g * HD;
-    const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+    Walk<HD> w;
+    w.t = run_begin(runs, blockIdx.x);
+    w.t_end = run_begin(runs, blockIdx.x + 1);
+    w.ei = sm.found;
+    w.e = entry(a.b, w.ei);
+    w.n_qt = row_tiles<HD>(a, w.e);
+    {
+        // the head, then the tile of rows, in which the run begins
+        unsigned each = 0;
+        for (int q = lane; q < w.n_qt; q += 32) each += rows_of<HD>(a, w.e, q).tiles;
 #pragma unroll
-    for (int i = 0; i < HD / 32; i++) out[lane + 32 * i] = T(acc[i] * inv);
-    if (a.lse && lane == 0) a.lse[(long long)t * a.n_q_heads + g] = m + logf(sum);
+        for (int d = 16; d; d >>= 1) each += __shfl_xor_sync(0xffffffffu, each, d);
+        const unsigned in = w.t - sm.found_t;
+        w.head = in / each;
+        const unsigned off = in - w.head * each;
+        unsigned pre = 0;
+        w.qt = 0;
+        w.unit_t = 0;
+        for (int base = 0; base < w.n_qt; base += 32) {
+            const unsigned x = base + lane < w.n_qt ? rows_of<HD>(a, w.e, base + lane).tiles : 0;
+            unsigned upto = x;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const unsigned o = __shfl_up_sync(0xffffffffu, upto, d);
+                if (lane >= d) upto += o;
+            }
+            const unsigned who = __ballot_sync(0xffffffffu, off >= pre + upto - x && off < pre + upto);
+            if (who) {
+                const int src = __ffs(who) - 1;
+                w.qt = base + src;
+                w.unit_t = w.t - (off - (pre + __shfl_sync(0xffffffffu, upto - x, src)));
+            }
+            pre += __shfl_sync(0xffffffffu, upto, 31);
+        }
+        w.r = rows_of<HD>(a, w.e, w.qt);
+    }
+
+    if (tid == 0) {
+        for (int i = 0; i < 2; i++) {
+            spb::mbar_init(spb::smem_u32(&sm.q_full[i]), 4);
+            spb::mbar_init(spb::smem_u32(&sm.k_full[i]), S::ConvWarps);
+            spb::mbar_init(spb::smem_u32(&sm.k_free[i]), 1);
+            spb::mbar_init(spb::smem_u32(&sm.v_full[i]), S::ConvWarps);
+            spb::mbar_init(spb::smem_u32(&sm.v_free[i]), 1);
+            spb::mbar_init(spb::smem_u32(&sm.s_full[i]), 1);
+            spb::mbar_init(spb::smem_u32(&sm.p_full[i]), 4);
+            spb::mbar_init(spb::smem_u32(&sm.pv_done[i]), 1);
+        }
+        spb::mbar_init(spb::smem_u32(&sm.end), 1);
+        spb::mbar_init_fence();
+        sm.abort = 0;
+    }
+    if (warp == kWarps - 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                     ::"r"(spb::smem_u32(&sm.tmem)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = sm.tmem;
+    auto wait1 = [&](unsigned long long &bar, unsigned n) {     // for the end of phase n
+        const uint32_t b = spb::smem_u32(&bar);
+        return spb::mbar_try_wait(b, n & 1) || wait_slow(b, n & 1, &sm.abort, a.b.status);
+    };
+    auto wait = [&](unsigned long long &bar, unsigned n) { return __all_sync(0xffffffffu, wait1(bar, n)) != 0; };
+
+    if (warp < S::SoftWarps) {
+        // ================= softmax: one thread for each row =================
+        const int i = warp >> 2, r = tid & 127;
+        const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
+        const uint32_t t_o = tmem + lanes + S::ColO + HD * i;
+        unsigned done = 0;                                      // tiles so far, of all units
+        for (; w.more(); w.next(a)) {
+            const int row = w.r.row0 + 128 * i + r;
+            const bool real = 128 * i + r < w.r.rows;
+            const int tok = w.e.q0 + row / a.group, qh = w.head * a.group + row % a.group;
+            const int first = w.e.kv_len - w.e.n, pos = first + row / a.group;
+            float mul = 0.0f;
+            // ---- the row of queries: scaled to fp16, dimensions in unpack4's order
+            {
+                const T *q = static_cast<const T *>(a.q) + (long long)tok * a.q_stride + qh * HD;
+                float top = 0.0f;
+                if (real) {
+#pragma unroll 4
+                    for (int d = 0; d < HD; d += 8) {
+                        const uint4 x = *reinterpret_cast<const uint4 *>(q + d);
+#pragma unroll
+                        for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(sp_load_as_float(reinterpret_cast<const T *>(&x), j)));
+                    }
+                }
+                float down, up;
+                row_scale(top, down, up);
+                mul = fabsf(a.scale) * kLog2e * up * (1.0f / Unit<FMT>::v);
+                if (a.scale < 0.0f) down = -down;
+                unsigned char *dst = sm.q[i] + (r >> 3) * (HD * 16) + (r & 7) * 16;
+#pragma unroll 4
+                for (int d = 0; d < HD; d += 8) {
+                    __half h[8];
+                    uint4 x = make_uint4(0u, 0u, 0u, 0u);
+                    if (real) x = *reinterpret_cast<const uint4 *>(q + d);
+#pragma unroll
+                    for (int j = 0; j < 8; j++)
+                        h[(j & 4) + ((j & 3) >> 1) + 2 * (j & 1)] =
+                            __float2half_rn(sp_load_as_float(reinterpret_cast<const T *>(&x), j) * down);
+                    *reinterpret_cast<uint4 *>(dst + (d >> 3) * 128) = *reinterpret_cast<const uint4 *>(h);
+                }
+                spb::fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) arrive(spb::smem_u32(&sm.q_full[i]));
+            }
+            const int hi = !real ? 0x7fffffff : a.causal ? pos : w.e.kv_len - 1;
+            const int lo = real && a.window > 0 ? pos - a.window + 1 : 0;
+            const long long slot = (long long)w.e.seq * a.l.heads + w.head;
+            const float *ksp = a.l.k_scale + slot * (a.l.max_seq >> a.l.block_log2);
+            const float *vsp = a.l.v_scale + slot * (a.l.max_seq >> a.l.block_log2);
+            float m = kNone, l = 0.0f;
+            const int k0 = w.k0(), k1 = w.k1();
+            for (int k = k0; k < k1; k++, done++) {
+                const int j0 = w.r.start + k * BN;
+                // a lane for each 16 positions: their scales (harmless ones past the end)
+                const int at = j0 + 16 * (lane % (BN / 16));
+                float ks = 0.0f, vs = 1.0f;
+                if (at < w.e.kv_len) {
+                    ks = ksp[at >> a.l.block_log2];
+                    vs = fmaxf(vsp[at >> a.l.block_log2], kScaleMin);
+                }
+                const float lv = lg2(vs), iv = __frcp_rn(vs), f = ks;
+                const bool all = __all_sync(0xffffffffu, j0 + BN - 1 <= hi && j0 >= lo);
+                const int buf = NQ == 2 ? i : (int)(done & 1);
+                const uint32_t t_s = tmem + lanes + (NQ == 2 ? 128 : 64) * buf;
+                if (!wait(sm.s_full[buf], NQ == 2 ? done : done >> 1)) goto out;
+                fence_after();
+                // ---- largest exponent
+                float top = kNone;
+#pragma unroll
+                for (int c = 0; c < BN; c += 32) {
+                    uint32_t v[32];
+                    tmem_ld32(t_s + c, v);
+                    wait_ld();
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const float fg = __shfl_sync(0xffffffffu, f, c / 16 + h) * mul, lg = __shfl_sync(0xffffffffu, lv, c / 16 + h);
+                        if (all) {
+                            float x = __uint_as_float(v[16 * h]);
+#pragma unroll
+                            for (int j = 1; j < 16; j++) x = fmaxf(x, __uint_as_float(v[16 * h + j]));
+                            top = fmaxf(top, fmaf(x, fg, lg));
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 16; j++) {
+                                const int p = j0 + c + 16 * h + j;
+                                const float x = fmaf(__uint_as_float(v[16 * h + j]), fg, lg);
+                                if (p <= hi && p >= lo) top = fmaxf(top, x);
+                            }
+                        }
+                    }
+                }
+                const bool raise = top > m + 8.0f;
+                if (__any_sync(0xffffffffu, raise)) {
+                    const float fix = raise ? ex2(m - top) : 1.0f;
+                    if (raise) m = top;
+                    l *= fix;
+                    if (k > k0) {
+                        // the products so far are in: the values that they summed shrink too
+                        if (!wait(sm.pv_done[i], done - 1)) goto out;
+                        fence_after();
+#pragma unroll 1
+                        for (int c = 0; c < HD; c += 32) {
+                            uint32_t v[32];
+                            tmem_ld32(t_o + c, v);
+                            wait_ld();
+#pragma unroll
+                            for (int j = 0; j < 32; j++) v[j] = __float_as_uint(__uint_as_float(v[j]) * fix);
+                            tmem_st32(t_o + c, v);
+                        }
+                        wait_st();
+                    }
+                }
+                // ---- weights
+#pragma unroll
+                for (int c = 0; c < BN; c += 32) {
+                    uint32_t v[32], p[16];
+                    tmem_ld32(t_s + c, v);
+                    wait_ld();
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const float fg = __shfl_sync(0xffffffffu, f, c / 16 + h) * mul;
+                        const float off = __shfl_sync(0xffffffffu, lv, c / 16 + h) - m;
+                        const float ig = __shfl_sync(0xffffffffu, iv, c / 16 + h);
+                        float sum = 0.0f;
+#pragma unroll
+                        for (int j = 0; j < 16; j += 2) {
+                            float x = fmaf(__uint_as_float(v[16 * h + j]), fg, off), y = fmaf(__uint_as_float(v[16 * h + j + 1]), fg, off);
+                            if (!all) {
+                                const int at = j0 + c + 16 * h + j;
+                                if (at > hi || at < lo) x = -INFINITY;
+                                if (at + 1 > hi || at + 1 < lo) y = -INFINITY;
+                            }
+                            x = ex2(x);
+                            y = ex2(y);
+                            sum += x + y;
+                            const __half2 hw = __floats2half2_rn(x, y);
+                            p[8 * h + j / 2] = *reinterpret_cast<const uint32_t *>(&hw);
+                        }
+                        l = fmaf(sum, ig, l);
+                    }
+                    tmem_st16(t_s + c / 2, p);
+                }
+                wait_st();
+                fence_before();
+                __syncwarp();
+                if (lane == 0) arrive(spb::smem_u32(&sm.p_full[buf]));
+            }
+            // ---- the unit's result, or this run's part of it
+            if (!wait(sm.pv_done[i], done - 1)) goto out;
+            fence_after();
+            const bool whole = k0 == 0 && k1 == w.r.tiles;
+            constexpr float kOut = 1.0f / Unit<FMT>::v;
+            if (whole) {
+                const float inv = l > 0.0f ? kOut / l : 0.0f;
+                T *out = static_cast<T *>(a.out) + (long long)tok * a.out_stride + qh * HD;
+#pragma unroll 1
+                for (int c = 0; c < HD; c += 32) {
+                    uint32_t v[32];
+                    tmem_ld32(t_o + c, v);
+                    wait_ld();
+                    if (real) {
+#pragma unroll
+                        for (int b = 0; b < 32; b += 8) {
+                            T x[8];
+#pragma unroll
+                            for (int j = 0; j < 8; j++)
+                                x[j] = T(__uint_as_float(v[b + (j & 4) + ((j & 3) >> 1) + 2 * (j & 1)]) * inv);
+                            *reinterpret_cast<uint4 *>(out + c + b) = *reinterpret_cast<const uint4 *>(x);
+                        }
+                    }
+                }
+                if (real && a.lse) a.lse[(long long)tok * a.n_q_heads + qh] = l > 0.0f ? kLn2 * (m + lg2(l)) : -INFINITY;
+            } else {
+                // rows side by side, so that a warp's stores are contiguous
+                float *part = a.partials + (long long)(2 * blockIdx.x + (w.unit_t >= run_begin(runs, blockIdx.x))) * S::SlotFloats;
+                const int prow = 128 * i + r;
+#pragma unroll 1
+                for (int c = 0; c < HD; c += 32) {
+                    uint32_t v[32];
+                    tmem_ld32(t_o + c, v);
+                    wait_ld();
+                    if (real) {
+#pragma unroll
+                        for (int b = 0; b < 32; b += 4)
+                            __stcg(reinterpret_cast<float4 *>(part) + (c + b) / 4 * S::ROWS + prow,
+                                   make_float4(__uint_as_float(v[b]), __uint_as_float(v[b + 2]), __uint_as_float(v[b + 1]),
+                                               __uint_as_float(v[b + 3])));
+                    }
+                }
+                if (real) __stcg(reinterpret_cast<float2 *>(part + S::ROWS * HD) + prow, make_float2(m, l));
+                if (tid == 0 && k0 == 0) {
+                    const unsigned last = w.unit_t + w.r.tiles - 1;
+                    *splits = {1, w.e.q0, w.r.row0, w.r.rows, w.head, w.unit_t, (unsigned)blockIdx.x, run_of_tile(runs, last)};
+                }
+            }
+            fence_before();
+        }
+    } else if (warp < S::SoftWarps + S::ConvWarps) {
+        // ================= codes to fp16 operands =================
+        // 16 codes a lane at a time: 8 positions x 4 runs of 16 dimensions, so
+        // that eight lanes' 16-byte stores fill a core matrix
+        const int cw = warp - S::SoftWarps;
+        constexpr int kLoads = BN * HD / 16 / (32 * S::ConvWarps);
+        constexpr int kSpan = HD / 64;                           // 64-dimension spans of a row
+        unsigned done = 0;
+        uint4 x[kLoads];
+        auto load = [&](const uint8_t *p) {
+#pragma unroll
+            for (int n = 0; n < kLoads; n++) {
+                const int u = cw + S::ConvWarps * n;             // (8 positions, 64 dimensions)
+                x[n] = *reinterpret_cast<const uint4 *>(p + (long long)(u / kSpan * 8 + (lane & 7)) * HD + u % kSpan * 64 + (lane >> 3) * 16);
+            }
+        };
+        auto store = [&](unsigned char *dst) {
+#pragma unroll
+            for (int n = 0; n < kLoads; n++) {
+                const int u = cw + S::ConvWarps * n;
+                unsigned char *d = dst + (u / kSpan) * (HD * 16) + (u % kSpan * 8 + (lane >> 3) * 2) * 128 + (lane & 7) * 16;
+                uint4 lo, hi;
+                unpack4<FMT>(x[n].x, lo.x, lo.y);
+                unpack4<FMT>(x[n].y, lo.z, lo.w);
+                unpack4<FMT>(x[n].z, hi.x, hi.y);
+                unpack4<FMT>(x[n].w, hi.z, hi.w);
+                *reinterpret_cast<uint4 *>(d) = lo;
+                *reinterpret_cast<uint4 *>(d + 128) = hi;
+            }
+        };
+        for (; w.more(); w.next(a)) {
+            const long long slot = (long long)w.e.seq * a.l.heads + w.head;
+            const uint8_t *kp = a.l.k + slot * a.l.max_seq * HD + (long long)w.r.start * HD;
+            const uint8_t *vp = a.l.v + slot * a.l.max_seq * HD + (long long)w.r.start * HD;
+            const int k0 = w.k0(), k1 = w.k1();
+            load(kp + (long long)k0 * BN * HD);
+            for (int k = k0; k < k1; k++, done++) {
+                const int st = done & 1;
+                if (done >= 2 && !wait(sm.k_free[st], done / 2 - 1)) goto out;
+                store(sm.k[st]);
+                load(vp + (long long)k * BN * HD);
+                spb::fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) arrive(spb::smem_u32(&sm.k_full[st]));
+                if (done >= 2 && !wait(sm.v_free[st], done / 2 - 1)) goto out;
+                store(sm.v[st]);
+                if (k + 1 < k1) load(kp + (long long)(k + 1) * BN * HD);
+                spb::fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) arrive(spb::smem_u32(&sm.v_full[st]));
+            }
+        }
+    } else if (lane == 0) {
+        // ================= the tensor cores' thread =================
+        unsigned done = 0, units = 0;
+        auto scores = [&](int i, unsigned n) {                   // tile n of the run, counted over all units
+            const uint32_t q = spb::smem_u32(sm.q[i]), k = spb::smem_u32(sm.k[n & 1]);
+            const uint32_t d = tmem + (NQ == 2 ? 128 * i : 64 * (n & 1));
+#pragma unroll
+            for (int s = 0; s < HD / 16; s++)
+                mma_ss(d, operand(q + s * 256, 128, HD * 16), operand(k + s * 256, 128, HD * 16), instr(BN, false), s > 0);
+            commit(spb::smem_u32(&sm.s_full[NQ == 2 ? i : n & 1]));
+        };
+        auto values = [&](int i, unsigned n, bool add) {
+            const uint32_t v = spb::smem_u32(sm.v[n & 1]);
+            const uint32_t p = tmem + (NQ == 2 ? 128 * i : 64 * (n & 1));
+#pragma unroll
+            for (int s = 0; s < BN / 16; s++)
+                mma_ts(tmem + S::ColO + HD * i, p + 8 * s, operand(v + s * 2 * (HD * 16), HD * 16, 128), instr(HD, true), add || s > 0);
+            commit(spb::smem_u32(&sm.pv_done[i]));
+        };
+        for (; w.more(); w.next(a), units++) {
+            const int n = w.k1() - w.k0();
+            if (!wait1(sm.k_full[done & 1], done / 2)) goto mma_out;
+            for (int i = 0; i < NQ; i++) {
+                if (!wait1(sm.q_full[i], units)) goto mma_out;
+                fence_after();
+                scores(i, done);
+            }
+            commit(spb::smem_u32(&sm.k_free[done & 1]));
+            for (int k = 0; k < n; k++, done++) {
+                if (k + 1 < n && !wait1(sm.k_full[(done + 1) & 1], (done + 1) / 2)) goto mma_out;
+                if (NQ == 1 && k + 1 < n) {
+                    fence_after();
+                    scores(0, done + 1);
+                    commit(spb::smem_u32(&sm.k_free[(done + 1) & 1]));
+                }
+                for (int i = 0; i < NQ; i++) {
+                    if (i == 0 && !wait1(sm.v_full[done & 1], done / 2)) goto mma_out;
+                    if (!wait1(sm.p_full[NQ == 2 ? i : done & 1], NQ == 2 ? done : done >> 1)) goto mma_out;
+                    fence_after();
+                    values(i, done, k > 0);
+                    if (NQ == 2 && k + 1 < n) scores(i, done + 1);
+                }
+                commit(spb::smem_u32(&sm.v_free[done & 1]));
+                if (NQ == 2 && k + 1 < n) commit(spb::smem_u32(&sm.k_free[(done + 1) & 1]));
+            }
+        }
+    mma_out:
+        // whatever was issued is over before tensor memory goes back
+        commit(spb::smem_u32(&sm.end));
+        spb::wait_stage(spb::smem_u32(&sm.end), 0, nullptr);
+    }
+out:
+    __syncwarp();
+    fence_before();
+    __syncthreads();
+    fence_after();
+    if (warp == kWarps - 1)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+}
+
+// Joins the parts of units that fell into several runs: block (i, y) the unit
+// that began in run i, 16 of the head's dimensions, a thread for each row.
+template <typename T, int FMT, int HD>
+__global__ void __launch_bounds__(Shape<HD>::ROWS) k_q8_attn_join(const __grid_constant__ AttnArgs a)
+{
+    using S = Shape<HD>;
+    const Split sp = reinterpret_cast<const Split *>(a.counters + kMaxCtas)[blockIdx.x];
+    const int row = threadIdx.x;
+    if (!sp.valid || row >= sp.rows) return;
+    float top = kNone, sum = 0.0f, acc[16];
+#pragma unroll
+    for (int j = 0; j < 16; j++) acc[j] = 0.0f;
+    for (unsigned r = sp.run0; r <= sp.run1; r++) {
+        const float *part = a.partials + (long long)(2 * r + (r == sp.run0)) * S::SlotFloats;
+        const float2 ml = __ldcg(reinterpret_cast<const float2 *>(part + S::ROWS * HD) + row);
+        float4 x[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) x[j] = __ldcg(reinterpret_cast<const float4 *>(part) + (4 * blockIdx.y + j) * S::ROWS + row);
+        const float up = fmaxf(top, ml.x), f0 = ex2(top - up), f1 = ex2(ml.x - up);
+        top = up;
+        sum = fmaf(ml.y, f1, sum * f0);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            acc[4 * j] = fmaf(x[j].x, f1, acc[4 * j] * f0);
+            acc[4 * j + 1] = fmaf(x[j].y, f1, acc[4 * j + 1] * f0);
+            acc[4 * j + 2] = fmaf(x[j].z, f1, acc[4 * j + 2] * f0);
+            acc[4 * j + 3] = fmaf(x[j].w, f1, acc[4 * j + 3] * f0);
+        }
+    }
+    const float inv = sum > 0.0f ? (1.0f / Unit<FMT>::v) / sum : 0.0f;
+    const int rr = sp.row0 + row, tok = sp.q0 + rr / a.group, qh = sp.head * a.group + rr % a.group;
+    T x[16];
+#pragma unroll
+    for (int j = 0; j < 16; j++) x[j] = T(acc[j] * inv);
+    T *out = static_cast<T *>(a.out) + (long long)tok * a.out_stride + qh * HD + 16 * blockIdx.y;
+    reinterpret_cast<uint4 *>(out)[0] = reinterpret_cast<const uint4 *>(x)[0];
+    reinterpret_cast<uint4 *>(out)[1] = reinterpret_cast<const uint4 *>(x)[1];
+    if (a.lse && blockIdx.y == 0) a.lse[(long long)tok * a.n_q_heads + qh] = sum > 0.0f ? kLn2 * (top + lg2(sum)) : -INFINITY;
+}
+
+template <typename T, int FMT, int HD>
+int launch(const AttnArgs &a, int sms, cudaStream_t s)
+{
+    using S = Shape<HD>;
+    auto kernel = k_q8_attn_many<T, FMT, HD>;
+    constexpr int smem = sizeof(ManySmem<HD>);
+    static std::atomic<unsigned long long> ready{0};      // devices whose attribute is set
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (!(ready.load(std::memory_order_acquire) >> (dev & 63) & 1)) {
+        const int rc = sp_check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
+                                     "q8_attn shared memory");
+        if (rc) return rc;
+        if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_release);
+    }
+    kernel<<<sms, S::Threads, smem, s>>>(a);
+    int rc = sp_check_cuda(cudaGetLastError(), "q8_attn launch");
+    if (rc) return rc;
+    k_q8_attn_join<T, FMT, HD><<<dim3(sms, HD / 16), S::ROWS, 0, s>>>(a);
+    return sp_check_cuda(cudaGetLastError(), "q8_attn join launch");
 }
 
 template <typename T, int FMT>
-void launch_rows(const AttnArgs &a, int hd, unsigned grid, cudaStream_t s)
+int launch_of(const AttnArgs &a, int hd, int sms, cudaStream_t s)
 {
-    if (hd == 64) k_q8_attn_rows<T, FMT, 64><<<grid, 128, 0, s>>>(a);
-    else if (hd == 128) k_q8_attn_rows<T, FMT, 128><<<grid, 128, 0, s>>>(a);
-    else k_q8_attn_rows<T, FMT, 256><<<grid, 128, 0, s>>>(a);
+    if (hd == 64) return launch<T, FMT, 64>(a, sms, s);
+    if (hd == 128) return launch<T, FMT, 128>(a, sms, s);
+    return launch<T, FMT, 256>(a, sms, s);
 }
 
 }  // namespace
 
 namespace q8 {
+size_t split_bytes(int sm_count) { return ((size_t)sm_count * sizeof(Split) + 255) / 256 * 256; }
+
 int launch_many(const AttnArgs &a, int format, int dtype, int hd, int sms, cudaStream_t s)
 {
-    (void)sms;
-    const long long units = (long long)a.b.n_tokens * a.n_q_heads;
-    if (units > 0x7fffffff) return sp_set_error(SP_ERR_ARG, "q8_attn: %lld rows in one call", units);
-    const unsigned grid = (unsigned)((units + 3) / 4);
-    if (dtype == SP_DTYPE_F16) {
-        if (format == SP_Q8_INT8) launch_rows<__half, SP_Q8_INT8>(a, hd, grid, s);
-        else launch_rows<__half, SP_Q8_E4M3>(a, hd, grid, s);
-    } else {
-        if (format == SP_Q8_INT8) launch_rows<__nv_bfloat16, SP_Q8_INT8>(a, hd, grid, s);
-        else launch_rows<__nv_bfloat16, SP_Q8_E4M3>(a, hd, grid, s);
-    }
-    return sp_check_cuda(cudaGetLastError(), "q8_attn launch");
+    if (dtype == SP_DTYPE_F16)
+        return format == SP_Q8_INT8 ? launch_of<__half, SP_Q8_INT8>(a, hd, sms, s) : launch_of<__half, SP_Q8_E4M3>(a, hd, sms, s);
+    return format == SP_Q8_INT8 ? launch_of<__nv_bfloat16, SP_Q8_INT8>(a, hd, sms, s)
+                                : launch_of<__nv_bfloat16, SP_Q8_E4M3>(a, hd, sms, s);
 }
 }  // namespace q8
