@@ -462,7 +462,10 @@ __global__ void __launch_bounds__(Shape<HD>::Threads, 1) k_q8_attn_many(const __
                 __syncwarp();
                 if (lane == 0) arrive(spb::smem_u32(&sm.p_full[buf]));
             }
-            // ---- the unit's result, or this run's part of it
+            // ---- the unit's result, or this run's part of it.  With two buffers of
+            // scores this warp may be two products ahead: a phase is waited for
+            // only after the one before it.
+            if (NQ == 1 && k1 - k0 > 1 && !wait(sm.pv_done[i], done - 2)) goto out;
             if (!wait(sm.pv_done[i], done - 1)) goto out;
             fence_after();
             const bool whole = k0 == 0 && k1 == w.r.tiles;
