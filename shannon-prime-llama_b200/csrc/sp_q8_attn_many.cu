@@ -8,7 +8,7 @@
 //     P = 2^(S f + log2 vs - m), by the rows' own threads, back into the
 //         columns of S as fp16 (the softmax of sp_q8_attn.cu)
 //     O += P V      P from tensor memory, V from shared memory
-// Codes become fp16 once for all 256 rows: eight warps load them, unpack them
+// Codes become fp16 once for all 256 rows: four warps (eight) load them, unpack them
 // in registers and store them in the core-matrix layout (8 rows of 16 bytes)
 // that serves K as the K-major and V as the MN-major operand.  One thread
 // issues the products; while a softmax warpgroup works on its 128 rows, the
@@ -17,6 +17,7 @@
 #include "sp_bulk.cuh"
 
 #include <atomic>
+#include <type_traits>
 
 namespace {
 
@@ -27,8 +28,8 @@ struct Shape {
     static constexpr int NQ = HD == 256 ? 1 : 2;       // 128-row tiles of queries
     static constexpr int BN = HD == 256 ? 64 : 128;    // positions of a tile
     static constexpr int ROWS = 128 * NQ;
-    static constexpr int SoftWarps = 4 * NQ, ConvWarps = 8;
-    static constexpr int Threads = 32 * (SoftWarps + ConvWarps + 1);
+    static constexpr int SoftWarps = 4 * NQ, ConvWarps = HD == 256 ? 8 : 4;
+    static constexpr int Threads = 32 * (SoftWarps + ConvWarps + 4);   // the last four: one issues the products
     static constexpr int ColO = 256;                   // S (and P) at 128 i or 64 (k & 1), O at 256 + HD i
     static constexpr int StageB = BN * HD * 2, QB = 128 * HD * 2;
     static constexpr int SlotFloats = ROWS * (HD + 2);
@@ -75,12 +76,46 @@ __device__ __forceinline__ void tmem_st32(uint32_t at, const uint32_t (&v)[32])
                  "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
                  ::"r"(at), Q8_R8(0), Q8_R8(8), Q8_R8(16), Q8_R8(24) : "memory");
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t at, uint32_t (&v)[16])
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+                   "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+                 : "r"(at));
+}
 __device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t (&v)[16])
 {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
                  ::"r"(at), Q8_R8(0), Q8_R8(8) : "memory");
 }
 #undef Q8_R8
+
+// Two 32-bit sums or products at a time, and the largest of three.
+struct F2 {
+    float x, y;
+};
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c)
+{
+    F2 d;
+    asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+        "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b)
+{
+    F2 d;
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+        "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c)
+{
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
 
 // Shared-memory operand without swizzle, in core matrices of 8 rows of 16
 // bytes: byte offsets between core matrices along and across the leading
@@ -119,7 +154,7 @@ __device__ __forceinline__ void arrive(uint32_t bar)
 }
 
 // Waits for a phase; false once any wait of this CTA has run out (2 s).
-__device__ __noinline__ bool wait_slow(uint32_t bar, uint32_t parity, int *abort, unsigned int *status)
+__device__ __forceinline__ bool wait_slow(uint32_t bar, uint32_t parity, int *abort, unsigned int *status)
 {
     const unsigned long long t0 = spb::global_ns();
     for (;;) {
@@ -300,7 +335,8 @@ __global__ void __launch_bounds__(Shape<HD>::Threads, 1) k_q8_attn_many(const __
         spb::mbar_init_fence();
         sm.abort = 0;
     }
-    if (warp == kWarps - 1) {
+    constexpr int kMmaWarp = S::SoftWarps + S::ConvWarps;
+    if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
                      ::"r"(spb::smem_u32(&sm.tmem)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -327,33 +363,44 @@ __global__ void __launch_bounds__(Shape<HD>::Threads, 1) k_q8_attn_many(const __
             const int tok = w.e.q0 + row / a.group, qh = w.head * a.group + row % a.group;
             const int first = w.e.kv_len - w.e.n, pos = first + row / a.group;
             float mul = 0.0f;
-            // ---- the row of queries: scaled to fp16, dimensions in unpack4's order
+            // ---- the rows of queries: a warp reads its 32 rows, 8 rows x 4 runs of 8
+            // dimensions at a time, scales each to fp16 and stores it with its
+            // dimensions in unpack4's order
             {
-                const T *q = static_cast<const T *>(a.q) + (long long)tok * a.q_stride + qh * HD;
-                float top = 0.0f;
-                if (real) {
-#pragma unroll 4
-                    for (int d = 0; d < HD; d += 8) {
-                        const uint4 x = *reinterpret_cast<const uint4 *>(q + d);
+#pragma unroll 1
+                for (int r8 = 0; r8 < 32; r8 += 8) {
+                    const int rr = 128 * i + 32 * (warp & 3) + r8 + (lane & 7);       // of the unit's rows
+                    const int ar = w.r.row0 + rr;
+                    const T *q = static_cast<const T *>(a.q) + (long long)(w.e.q0 + ar / a.group) * a.q_stride +
+                                 (w.head * a.group + ar % a.group) * HD + (lane >> 3) * 8;
+                    uint4 x[HD / 32];
 #pragma unroll
-                        for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(sp_load_as_float(reinterpret_cast<const T *>(&x), j)));
+                    for (int n = 0; n < HD / 32; n++) {
+                        x[n] = make_uint4(0u, 0u, 0u, 0u);
+                        if (rr < w.r.rows) x[n] = *reinterpret_cast<const uint4 *>(q + 32 * n);
                     }
-                }
-                float down, up;
-                row_scale(top, down, up);
-                mul = fabsf(a.scale) * kLog2e * up * (1.0f / Unit<FMT>::v);
-                if (a.scale < 0.0f) down = -down;
-                unsigned char *dst = sm.q[i] + (r >> 3) * (HD * 16) + (r & 7) * 16;
-#pragma unroll 4
-                for (int d = 0; d < HD; d += 8) {
-                    __half h[8];
-                    uint4 x = make_uint4(0u, 0u, 0u, 0u);
-                    if (real) x = *reinterpret_cast<const uint4 *>(q + d);
+                    float top = 0.0f;
 #pragma unroll
-                    for (int j = 0; j < 8; j++)
-                        h[(j & 4) + ((j & 3) >> 1) + 2 * (j & 1)] =
-                            __float2half_rn(sp_load_as_float(reinterpret_cast<const T *>(&x), j) * down);
-                    *reinterpret_cast<uint4 *>(dst + (d >> 3) * 128) = *reinterpret_cast<const uint4 *>(h);
+                    for (int n = 0; n < HD / 32; n++)
+#pragma unroll
+                        for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(sp_load_as_float(reinterpret_cast<const T *>(&x[n]), j)));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                    float down, up;
+                    row_scale(top, down, up);
+                    up = __shfl_sync(0xffffffffu, up, lane & 7);
+                    if ((lane & ~7) == r8) mul = fabsf(a.scale) * kLog2e * up * (1.0f / Unit<FMT>::v);
+                    if (a.scale < 0.0f) down = -down;
+                    unsigned char *dst = sm.q[i] + ((rr & 127) >> 3) * (HD * 16) + (lane >> 3) * 128 + (lane & 7) * 16;
+#pragma unroll
+                    for (int n = 0; n < HD / 32; n++) {
+                        __half h[8];
+#pragma unroll
+                        for (int j = 0; j < 8; j++)
+                            h[(j & 4) + ((j & 3) >> 1) + 2 * (j & 1)] =
+                                __float2half_rn(sp_load_as_float(reinterpret_cast<const T *>(&x[n]), j) * down);
+                        *reinterpret_cast<uint4 *>(dst + 512 * n) = *reinterpret_cast<const uint4 *>(h);
+                    }
                 }
                 spb::fence_proxy_async();
                 __syncwarp();
@@ -366,96 +413,109 @@ __global__ void __launch_bounds__(Shape<HD>::Threads, 1) k_q8_attn_many(const __
             const float *vsp = a.l.v_scale + slot * (a.l.max_seq >> a.l.block_log2);
             float m = kNone, l = 0.0f;
             const int k0 = w.k0(), k1 = w.k1();
+            // a lane for each 16 positions of a tile: their scales, loaded a tile
+            // ahead (harmless ones past the end)
+            float ks = 0.0f, vs = 1.0f;
+            auto load_scales = [&](int k) {
+                const int at = w.r.start + k * BN + 16 * (lane % (BN / 16));
+                const bool in = at < w.e.kv_len;
+                ks = in ? ksp[at >> a.l.block_log2] : 0.0f;
+                vs = in ? vsp[at >> a.l.block_log2] : 1.0f;
+            };
+            load_scales(k0);
             for (int k = k0; k < k1; k++, done++) {
                 const int j0 = w.r.start + k * BN;
-                // a lane for each 16 positions: their scales (harmless ones past the end)
-                const int at = j0 + 16 * (lane % (BN / 16));
-                float ks = 0.0f, vs = 1.0f;
-                if (at < w.e.kv_len) {
-                    ks = ksp[at >> a.l.block_log2];
-                    vs = fmaxf(vsp[at >> a.l.block_log2], kScaleMin);
-                }
-                const float lv = lg2(vs), iv = __frcp_rn(vs), f = ks;
+                const float vc = fmaxf(vs, kScaleMin), lv = lg2(vc), iv = __frcp_rn(vc), f = ks;
+                if (k + 1 < k1) load_scales(k + 1);
                 const bool all = __all_sync(0xffffffffu, j0 + BN - 1 <= hi && j0 >= lo);
                 const int buf = NQ == 2 ? i : (int)(done & 1);
                 const uint32_t t_s = tmem + lanes + (NQ == 2 ? 128 : 64) * buf;
                 if (!wait(sm.s_full[buf], NQ == 2 ? done : done >> 1)) goto out;
                 fence_after();
-                // ---- largest exponent
-                float top = kNone;
+                uint32_t p[BN / 2];
+                float sum = 0.0f, over = 0.0f;
+                // ---- weights relative to the maximum so far; over: the largest exponent
+                auto weights = [&](auto masked) {
+                    uint32_t v[2][16];
+                    tmem_ld16(t_s, v[0]);
+                    sum = 0.0f;
+                    over = -INFINITY;
 #pragma unroll
-                for (int c = 0; c < BN; c += 32) {
-                    uint32_t v[32];
-                    tmem_ld32(t_s + c, v);
-                    wait_ld();
-#pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        const float fg = __shfl_sync(0xffffffffu, f, c / 16 + h) * mul, lg = __shfl_sync(0xffffffffu, lv, c / 16 + h);
-                        if (all) {
-                            float x = __uint_as_float(v[16 * h]);
-#pragma unroll
-                            for (int j = 1; j < 16; j++) x = fmaxf(x, __uint_as_float(v[16 * h + j]));
-                            top = fmaxf(top, fmaf(x, fg, lg));
-                        } else {
-#pragma unroll
-                            for (int j = 0; j < 16; j++) {
-                                const int p = j0 + c + 16 * h + j;
-                                const float x = fmaf(__uint_as_float(v[16 * h + j]), fg, lg);
-                                if (p <= hi && p >= lo) top = fmaxf(top, x);
-                            }
-                        }
-                    }
-                }
-                const bool raise = top > m + 8.0f;
-                if (__any_sync(0xffffffffu, raise)) {
-                    const float fix = raise ? ex2(m - top) : 1.0f;
-                    if (raise) m = top;
-                    l *= fix;
-                    if (k > k0) {
-                        // the products so far are in: the values that they summed shrink too
-                        if (!wait(sm.pv_done[i], done - 1)) goto out;
-                        fence_after();
-#pragma unroll 1
-                        for (int c = 0; c < HD; c += 32) {
-                            uint32_t v[32];
-                            tmem_ld32(t_o + c, v);
-                            wait_ld();
-#pragma unroll
-                            for (int j = 0; j < 32; j++) v[j] = __float_as_uint(__uint_as_float(v[j]) * fix);
-                            tmem_st32(t_o + c, v);
-                        }
-                        wait_st();
-                    }
-                }
-                // ---- weights
-#pragma unroll
-                for (int c = 0; c < BN; c += 32) {
-                    uint32_t v[32], p[16];
-                    tmem_ld32(t_s + c, v);
-                    wait_ld();
-#pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        const float fg = __shfl_sync(0xffffffffu, f, c / 16 + h) * mul;
-                        const float off = __shfl_sync(0xffffffffu, lv, c / 16 + h) - m;
-                        const float ig = __shfl_sync(0xffffffffu, iv, c / 16 + h);
-                        float sum = 0.0f;
+                    for (int c = 0; c < BN / 16; c++) {
+                        const float fg = __shfl_sync(0xffffffffu, f, c) * mul;
+                        const float off = __shfl_sync(0xffffffffu, lv, c) - m, ig = __shfl_sync(0xffffffffu, iv, c);
+                        wait_ld();
+                        if (c + 1 < BN / 16) tmem_ld16(t_s + 16 * (c + 1), v[(c + 1) & 1]);
+                        const uint32_t(&u)[16] = v[c & 1];
+                        F2 part = {0.0f, 0.0f};
 #pragma unroll
                         for (int j = 0; j < 16; j += 2) {
-                            float x = fmaf(__uint_as_float(v[16 * h + j]), fg, off), y = fmaf(__uint_as_float(v[16 * h + j + 1]), fg, off);
-                            if (!all) {
-                                const int at = j0 + c + 16 * h + j;
-                                if (at > hi || at < lo) x = -INFINITY;
-                                if (at + 1 > hi || at + 1 < lo) y = -INFINITY;
+                            F2 x = fma2({__uint_as_float(u[j]), __uint_as_float(u[j + 1])}, {fg, fg}, {off, off});
+                            if (decltype(masked)::value) {
+                                const int at = j0 + 16 * c + j;
+                                if (at > hi || at < lo) x.x = -INFINITY;
+                                if (at + 1 > hi || at + 1 < lo) x.y = -INFINITY;
                             }
-                            x = ex2(x);
-                            y = ex2(y);
-                            sum += x + y;
-                            const __half2 hw = __floats2half2_rn(x, y);
-                            p[8 * h + j / 2] = *reinterpret_cast<const uint32_t *>(&hw);
+                            over = max3(over, x.x, x.y);
+                            x.x = ex2(x.x);
+                            x.y = ex2(x.y);
+                            part = add2(part, x);
+                            const __half2 hw = __floats2half2_rn(x.x, x.y);
+                            p[8 * c + j / 2] = *reinterpret_cast<const uint32_t *>(&hw);
                         }
-                        l = fmaf(sum, ig, l);
+                        sum = fmaf(part.x + part.y, ig, sum);
                     }
-                    tmem_st16(t_s + c / 2, p);
+                };
+                // ---- a row's first tile, and one whose scores pass the maximum by more
+                // than 2^8: the maximum is found before the weights are taken
+                auto raise = [&]() {
+                    float top = kNone;
+#pragma unroll 1
+                    for (int c = 0; c < BN / 16; c++) {
+                        const float fg = __shfl_sync(0xffffffffu, f, c) * mul, lg = __shfl_sync(0xffffffffu, lv, c);
+                        uint32_t v[16];
+                        tmem_ld16(t_s + 16 * c, v);
+                        wait_ld();
+#pragma unroll
+                        for (int j = 0; j < 16; j++) {
+                            const int at = j0 + 16 * c + j;
+                            if (at <= hi && at >= lo) top = fmaxf(top, fmaf(__uint_as_float(v[j]), fg, lg));
+                        }
+                    }
+                    const bool up = top > m + 8.0f;
+                    const float fix = up ? ex2(m - top) : 1.0f;
+                    if (up) m = top;
+                    l *= fix;
+                    if (k == k0) return true;
+                    // the products so far are in: the values that they summed shrink too
+                    if (!wait(sm.pv_done[i], done - 1)) return false;
+                    fence_after();
+#pragma unroll 1
+                    for (int c = 0; c < HD; c += 16) {
+                        uint32_t v[16];
+                        tmem_ld16(t_o + c, v);
+                        wait_ld();
+#pragma unroll
+                        for (int j = 0; j < 16; j++) v[j] = __float_as_uint(__uint_as_float(v[j]) * fix);
+                        tmem_st16(t_o + c, v);
+                    }
+                    wait_st();
+                    return true;
+                };
+                bool fresh = k == k0;
+                for (;;) {
+                    if (fresh && !raise()) goto out;
+                    if (all) weights(std::false_type{});
+                    else weights(std::true_type{});
+                    if (fresh || !__any_sync(0xffffffffu, over > 8.0f)) break;
+                    fresh = true;
+                }
+                l += sum;
+                if constexpr (BN == 128) {
+                    tmem_st32(t_s, reinterpret_cast<const uint32_t(&)[32]>(p[0]));
+                    tmem_st32(t_s + 32, reinterpret_cast<const uint32_t(&)[32]>(p[32]));
+                } else {
+                    tmem_st32(t_s, reinterpret_cast<const uint32_t(&)[32]>(p[0]));
                 }
                 wait_st();
                 fence_before();
@@ -523,15 +583,15 @@ __global__ void __launch_bounds__(Shape<HD>::Threads, 1) k_q8_attn_many(const __
         constexpr int kLoads = BN * HD / 16 / (32 * S::ConvWarps);
         constexpr int kSpan = HD / 64;                           // 64-dimension spans of a row
         unsigned done = 0;
-        uint4 x[kLoads];
-        auto load = [&](const uint8_t *p) {
+        uint4 kx[kLoads], vx[kLoads];                            // each loaded a tile ahead
+        auto load = [&](uint4(&x)[kLoads], const uint8_t *p) {
 #pragma unroll
             for (int n = 0; n < kLoads; n++) {
                 const int u = cw + S::ConvWarps * n;             // (8 positions, 64 dimensions)
                 x[n] = *reinterpret_cast<const uint4 *>(p + (long long)(u / kSpan * 8 + (lane & 7)) * HD + u % kSpan * 64 + (lane >> 3) * 16);
             }
         };
-        auto store = [&](unsigned char *dst) {
+        auto store = [&](const uint4(&x)[kLoads], unsigned char *dst, unsigned long long &full) {
 #pragma unroll
             for (int n = 0; n < kLoads; n++) {
                 const int u = cw + S::ConvWarps * n;
@@ -544,30 +604,28 @@ __global__ void __launch_bounds__(Shape<HD>::Threads, 1) k_q8_attn_many(const __
                 *reinterpret_cast<uint4 *>(d) = lo;
                 *reinterpret_cast<uint4 *>(d + 128) = hi;
             }
+            spb::fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) arrive(spb::smem_u32(&full));
         };
         for (; w.more(); w.next(a)) {
             const long long slot = (long long)w.e.seq * a.l.heads + w.head;
             const uint8_t *kp = a.l.k + slot * a.l.max_seq * HD + (long long)w.r.start * HD;
             const uint8_t *vp = a.l.v + slot * a.l.max_seq * HD + (long long)w.r.start * HD;
             const int k0 = w.k0(), k1 = w.k1();
-            load(kp + (long long)k0 * BN * HD);
+            load(kx, kp + (long long)k0 * BN * HD);
+            load(vx, vp + (long long)k0 * BN * HD);
             for (int k = k0; k < k1; k++, done++) {
                 const int st = done & 1;
                 if (done >= 2 && !wait(sm.k_free[st], done / 2 - 1)) goto out;
-                store(sm.k[st]);
-                load(vp + (long long)k * BN * HD);
-                spb::fence_proxy_async();
-                __syncwarp();
-                if (lane == 0) arrive(spb::smem_u32(&sm.k_full[st]));
+                store(kx, sm.k[st], sm.k_full[st]);
+                if (k + 1 < k1) load(kx, kp + (long long)(k + 1) * BN * HD);
                 if (done >= 2 && !wait(sm.v_free[st], done / 2 - 1)) goto out;
-                store(sm.v[st]);
-                if (k + 1 < k1) load(kp + (long long)(k + 1) * BN * HD);
-                spb::fence_proxy_async();
-                __syncwarp();
-                if (lane == 0) arrive(spb::smem_u32(&sm.v_full[st]));
+                store(vx, sm.v[st], sm.v_full[st]);
+                if (k + 1 < k1) load(vx, vp + (long long)(k + 1) * BN * HD);
             }
         }
-    } else if (lane == 0) {
+    } else if (warp == kMmaWarp && lane == 0) {
         // ================= the tensor cores' thread =================
         unsigned done = 0, units = 0;
         auto scores = [&](int i, unsigned n) {                   // tile n of the run, counted over all units
@@ -623,7 +681,7 @@ out:
     fence_before();
     __syncthreads();
     fence_after();
-    if (warp == kWarps - 1)
+    if (warp == kMmaWarp)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
 }
 
