@@ -183,6 +183,15 @@ __global__ void __launch_bounds__(kThreads, CTAS) k_q8_attn_few(const __grid_con
                     }
                 }
             }
+            // codes past the end may be NaN, which a weight of 0 does not undo
+            if (FMT == SP_Q8_E4M3 && j0 + 15 >= e.kv_len) {
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    if (j0 + 2 * c + (r & 1) + 8 * (r >> 1) >= e.kv_len) {
+#pragma unroll
+                        for (int i = 0; i < VW; i++) vw[r][i] = 0;
+                    }
+            }
             vs = vsp[j0 >> a.l.block_log2];
         };
         // dimension of code word i of a V row
@@ -216,9 +225,8 @@ __global__ void __launch_bounds__(kThreads, CTAS) k_q8_attn_few(const __grid_con
             if (lane == 0) sm.up[row] = up;
 #pragma unroll
             for (int i = 0; i < E; i++) {
-                const int d = lane + 32 * i, s = d / 64 * 4 + d % 16 / 4, p = d % 4;
-                // word order (0, 2), (1, 3): unpack4's pairs
-                reinterpret_cast<__half *>(&sm.q[n][s][4 * warp + d % 64 / 16])[(p >> 1) + 2 * (p & 1)] = __float2half_rn(x[i] * down);
+                const int d = lane + 32 * i, s = d / 64 * 4 + d % 16 / 4;
+                reinterpret_cast<__half *>(&sm.q[n][s][4 * warp + d % 64 / 16])[d % 4] = __float2half_rn(x[i] * down);
             }
         }
         __syncthreads();
@@ -239,7 +247,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) k_q8_attn_few(const __grid_con
 #pragma unroll
             for (int i = 0; i < 2; i++) {
                 const int row = 8 * n + 2 * c + i, pos = first + row / G;
-                mul[n][i] = a.scale * kLog2e * sm.up[row] * (1.0f / Unit<FMT>::v);
+                mul[n][i] = a.scale * kLog2e * sm.up[row];
                 hi[n][i] = a.causal ? pos : e.kv_len - 1;
                 lo[n][i] = a.window > 0 ? pos - a.window + 1 : 0;
                 m[n][i] = kNone;
@@ -333,7 +341,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) k_q8_attn_few(const __grid_con
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
                     uint32_t f[4];
-                    const unsigned pick = h ? 0x7632 : 0x5410;
+                    const unsigned pick = h ? 0x7362 : 0x5140;     // a dimension of two positions side by side
                     unpack4<FMT>(__byte_perm(vw[0][i], vw[1][i], pick), f[0], f[1]);
                     unpack4<FMT>(__byte_perm(vw[2][i], vw[3][i], pick), f[2], f[3]);
 #pragma unroll
@@ -395,9 +403,8 @@ __global__ void __launch_bounds__(kThreads, CTAS) k_q8_attn_few(const __grid_con
         const bool whole = k0 == 0 && k1 == u.tiles;
         const unsigned run0 = run_of_tile(runs, unit_t), run1 = run_of_tile(runs, unit_t + u.tiles - 1);
         constexpr int kSlot = 8 * NT * (HD + 2);
-        constexpr float kOut = 1.0f / Unit<FMT>::v;
         auto finish = [&](int row, int d, float4 v, float top, float sum) {
-            const float inv = sum > 0.0f ? kOut / sum : 0.0f;
+            const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
             T w[4] = {T(v.x * inv), T(v.y * inv), T(v.z * inv), T(v.w * inv)};
             const long long tok = e.q0 + row / G;
             const int qh = head * G + row % G;

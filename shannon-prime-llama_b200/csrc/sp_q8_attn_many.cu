@@ -8,7 +8,7 @@
 //     P = 2^(S f + log2 vs - m), by the rows' own threads, back into the
 //         columns of S as fp16 (the softmax of sp_q8_attn.cu)
 //     O += P V      P from tensor memory, V from shared memory
-// Codes become fp16 once for all 256 rows: four warps (eight) load them, unpack them
+// Codes become fp16 once for all 256 rows: seven warps (eleven) load them, unpack them
 // in registers and store them in the core-matrix layout (8 rows of 16 bytes)
 // that serves K as the K-major and V as the MN-major operand.  One thread
 // issues the products; while a softmax warpgroup works on its 128 rows, the
@@ -28,8 +28,8 @@ struct Shape {
     static constexpr int NQ = HD == 256 ? 1 : 2;       // 128-row tiles of queries
     static constexpr int BN = HD == 256 ? 64 : 128;    // positions of a tile
     static constexpr int ROWS = 128 * NQ;
-    static constexpr int SoftWarps = 4 * NQ, ConvWarps = HD == 256 ? 8 : 4;
-    static constexpr int Threads = 32 * (SoftWarps + ConvWarps + 4);   // the last four: one issues the products
+    static constexpr int SoftWarps = 4 * NQ, ConvWarps = 15 - SoftWarps;
+    static constexpr int Threads = 32 * (SoftWarps + ConvWarps + 1);   // the last warp issues the products
     static constexpr int ColO = 256;                   // S (and P) at 128 i or 64 (k & 1), O at 256 + HD i
     static constexpr int StageB = BN * HD * 2, QB = 128 * HD * 2;
     static constexpr int SlotFloats = ROWS * (HD + 2);
@@ -58,7 +58,6 @@ struct Split {
 // --- tensor core and tensor memory --------------------------------------
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 #define Q8_R8(b) "=r"(v[b]), "=r"(v[b + 1]), "=r"(v[b + 2]), "=r"(v[b + 3]), "=r"(v[b + 4]), "=r"(v[b + 5]), "=r"(v[b + 6]), "=r"(v[b + 7])
@@ -70,12 +69,6 @@ __device__ __forceinline__ void tmem_ld32(uint32_t at, uint32_t (&v)[32])
 }
 #undef Q8_R8
 #define Q8_R8(b) "r"(v[b]), "r"(v[b + 1]), "r"(v[b + 2]), "r"(v[b + 3]), "r"(v[b + 4]), "r"(v[b + 5]), "r"(v[b + 6]), "r"(v[b + 7])
-__device__ __forceinline__ void tmem_st32(uint32_t at, const uint32_t (&v)[32])
-{
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
-                 "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
-                 ::"r"(at), Q8_R8(0), Q8_R8(8), Q8_R8(16), Q8_R8(24) : "memory");
-}
 __device__ __forceinline__ void tmem_ld16(uint32_t at, uint32_t (&v)[16])
 {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
@@ -90,7 +83,20 @@ __device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t (&v)[16])
 }
 #undef Q8_R8
 
-// Two 32-bit sums or products at a time, and the largest of three.
+// Waits for the loads so far; their registers are named so that no use of them
+// moves before the wait.
+#define Q8_R8(b) "+r"(v[b]), "+r"(v[b + 1]), "+r"(v[b + 2]), "+r"(v[b + 3]), "+r"(v[b + 4]), "+r"(v[b + 5]), "+r"(v[b + 6]), "+r"(v[b + 7])
+__device__ __forceinline__ void wait_ld16(uint32_t (&v)[16])
+{
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : Q8_R8(0), Q8_R8(8) :: "memory");
+}
+__device__ __forceinline__ void wait_ld32(uint32_t (&v)[32])
+{
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : Q8_R8(0), Q8_R8(8), Q8_R8(16), Q8_R8(24) :: "memory");
+}
+#undef Q8_R8
+
+// Two 32-bit sums or products at a time.
 struct F2 {
     float x, y;
 };
@@ -110,11 +116,22 @@ __device__ __forceinline__ F2 add2(F2 a, F2 b)
         : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
     return d;
 }
-__device__ __forceinline__ float max3(float a, float b, float c)
+// 2^x for x >= -126 (below: 2^-126) without the special-function unit: the
+// nearest whole number n by adding and taking off 1.5 * 2^23, whose low bits
+// then are n and go to the exponent; 2^(x - n) by the polynomial of degree 4
+// with the least largest relative error on [-1/2, 1/2], 2.7e-6 (Remez exchange).
+__device__ __forceinline__ F2 exp2_poly(F2 x)
 {
-    float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-    return d;
+    constexpr float kRound = 12582912.0f;
+    x.x = fmaxf(x.x, -126.0f);
+    x.y = fmaxf(x.y, -126.0f);
+    const F2 t = add2(x, {kRound, kRound}), n = add2(t, {-kRound, -kRound}), r = fma2(n, {-1.0f, -1.0f}, x);
+    F2 p = fma2({0x1.3997d6p-7f, 0x1.3997d6p-7f}, r, {0x1.ca1444p-5f, 0x1.ca1444p-5f});
+    p = fma2(p, r, {0x1.ec06dap-3f, 0x1.ec06dap-3f});
+    p = fma2(p, r, {0x1.62e0dcp-1f, 0x1.62e0dcp-1f});
+    p = fma2(p, r, {0x1.ffffe8p-1f, 0x1.ffffe8p-1f});
+    return {__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)),
+            __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23))};
 }
 
 // Shared-memory operand without swizzle, in core matrices of 8 rows of 16
@@ -127,26 +144,29 @@ __device__ __forceinline__ uint64_t operand(uint32_t addr, uint32_t lbo, uint32_
            (uint64_t)((sbo >> 4) & 0x3FFFu) << 32 | (uint64_t)1 << 46;
 }
 
-// fp16 x fp16 -> fp32, M = 128
+// fp16 x fp16 -> fp32, M = 128.  A whole warp comes here and one elected lane
+// issues: the operands then stay in uniform registers (65 cycles for a product
+// of 128 x 128 x 16, against 122 to 200 from inside a one-lane branch).
 constexpr uint32_t instr(int n, bool b_mn)
 {
     return (1u << 4) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 }
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t i, uint32_t add)
 {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %3, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %4, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(add), "r"(i)
+    asm volatile("{\n\t.reg .pred p, e;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %3, 0;\n\t"
+                 "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %4, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(add), "r"(i)
                  : "memory");
 }
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t i, uint32_t add)
 {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %3, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %4, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(add), "r"(i)
+    asm volatile("{\n\t.reg .pred p, e;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %3, 0;\n\t"
+                 "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %4, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(add), "r"(i)
                  : "memory");
 }
 __device__ __forceinline__ void commit(uint32_t bar)
 {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+    asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+                 "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void arrive(uint32_t bar)
 {
@@ -224,6 +244,9 @@ struct Walk {
     }
 };
 
+// Which pairs of eight take the polynomial.
+__host__ __device__ constexpr bool kPoly(int j) { return j % 8 == 7; }
+
 template <typename T, int FMT, int HD>
 __global__ void __launch_bounds__(Shape<HD>::Threads, 1) k_q8_attn_many(const __grid_constant__ AttnArgs a)
 {
@@ -231,7 +254,7 @@ __global__ void __launch_bounds__(Shape<HD>::Threads, 1) k_q8_attn_many(const __
     constexpr int NQ = S::NQ, BN = S::BN;
     extern __shared__ __align__(128) unsigned char smem_raw[];
     ManySmem<HD> &sm = *reinterpret_cast<ManySmem<HD> *>(smem_raw);
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     constexpr int kWarps = S::Threads / 32;
     Split *splits = reinterpret_cast<Split *>(a.counters + kMaxCtas) + blockIdx.x;
     if (tid == 0) splits->valid = 0;
@@ -344,12 +367,11 @@ __global__ void __launch_bounds__(Shape<HD>::Threads, 1) k_q8_attn_many(const __
     fence_before();
     __syncthreads();
     fence_after();
-    const uint32_t tmem = sm.tmem;
-    auto wait1 = [&](unsigned long long &bar, unsigned n) {     // for the end of phase n
+    const uint32_t tmem = __shfl_sync(0xffffffffu, sm.tmem, 0);
+    auto wait = [&](unsigned long long &bar, unsigned n) {      // a whole warp, for the end of phase n
         const uint32_t b = spb::smem_u32(&bar);
-        return spb::mbar_try_wait(b, n & 1) || wait_slow(b, n & 1, &sm.abort, a.b.status);
+        return __all_sync(0xffffffffu, spb::mbar_try_wait(b, n & 1) || wait_slow(b, n & 1, &sm.abort, a.b.status)) != 0;
     };
-    auto wait = [&](unsigned long long &bar, unsigned n) { return __all_sync(0xffffffffu, wait1(bar, n)) != 0; };
 
     if (warp < S::SoftWarps) {
         // ================= softmax: one thread for each row =================
@@ -357,55 +379,58 @@ __global__ void __launch_bounds__(Shape<HD>::Threads, 1) k_q8_attn_many(const __
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
         const uint32_t t_o = tmem + lanes + S::ColO + HD * i;
         unsigned done = 0;                                      // tiles so far, of all units
+        // For the values of tile n.  With two buffers of scores a warp may be two
+        // products ahead of the tensor cores, and a barrier tells only neighbouring
+        // phases apart: the buffers have a barrier each.
+        auto wait_values = [&](unsigned n) { return NQ == 2 ? wait(sm.pv_done[i], n) : wait(sm.pv_done[n & 1], n >> 1); };
         for (; w.more(); w.next(a)) {
             const int row = w.r.row0 + 128 * i + r;
             const bool real = 128 * i + r < w.r.rows;
             const int tok = w.e.q0 + row / a.group, qh = w.head * a.group + row % a.group;
             const int first = w.e.kv_len - w.e.n, pos = first + row / a.group;
-            float mul = 0.0f;
-            // ---- the rows of queries: a warp reads its 32 rows, 8 rows x 4 runs of 8
-            // dimensions at a time, scales each to fp16 and stores it with its
-            // dimensions in unpack4's order
-            {
+            // ---- the warp's 32 rows of queries, 8 rows x 4 runs of 8 dimensions at a
+            // time, into the operand's places as they are; then a thread for each
+            // row scales its own to fp16
+            float mul, top = 0.0f;
+            unsigned char *own = sm.q[i] + (warp & 3) * 4 * (HD * 16);
 #pragma unroll 1
-                for (int r8 = 0; r8 < 32; r8 += 8) {
-                    const int rr = 128 * i + 32 * (warp & 3) + r8 + (lane & 7);       // of the unit's rows
-                    const int ar = w.r.row0 + rr;
-                    const T *q = static_cast<const T *>(a.q) + (long long)(w.e.q0 + ar / a.group) * a.q_stride +
-                                 (w.head * a.group + ar % a.group) * HD + (lane >> 3) * 8;
-                    uint4 x[HD / 32];
+            for (int n = 0; n < 4; n++) {
+                const int rr = 128 * i + 32 * (warp & 3) + 8 * n + (lane & 7), ar = w.r.row0 + rr;
+                const T *q = static_cast<const T *>(a.q) + (long long)(w.e.q0 + ar / a.group) * a.q_stride +
+                             (w.head * a.group + ar % a.group) * HD + (lane >> 3) * 8;
+                const uint32_t dst = spb::smem_u32(own + n * (HD * 16) + lane * 16), bytes = rr < w.r.rows ? 16 : 0;
 #pragma unroll
-                    for (int n = 0; n < HD / 32; n++) {
-                        x[n] = make_uint4(0u, 0u, 0u, 0u);
-                        if (rr < w.r.rows) x[n] = *reinterpret_cast<const uint4 *>(q + 32 * n);
-                    }
-                    float top = 0.0f;
-#pragma unroll
-                    for (int n = 0; n < HD / 32; n++)
-#pragma unroll
-                        for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(sp_load_as_float(reinterpret_cast<const T *>(&x[n]), j)));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-                    float down, up;
-                    row_scale(top, down, up);
-                    up = __shfl_sync(0xffffffffu, up, lane & 7);
-                    if ((lane & ~7) == r8) mul = fabsf(a.scale) * kLog2e * up * (1.0f / Unit<FMT>::v);
-                    if (a.scale < 0.0f) down = -down;
-                    unsigned char *dst = sm.q[i] + ((rr & 127) >> 3) * (HD * 16) + (lane >> 3) * 128 + (lane & 7) * 16;
-#pragma unroll
-                    for (int n = 0; n < HD / 32; n++) {
-                        __half h[8];
-#pragma unroll
-                        for (int j = 0; j < 8; j++)
-                            h[(j & 4) + ((j & 3) >> 1) + 2 * (j & 1)] =
-                                __float2half_rn(sp_load_as_float(reinterpret_cast<const T *>(&x[n]), j) * down);
-                        *reinterpret_cast<uint4 *>(dst + 512 * n) = *reinterpret_cast<const uint4 *>(h);
-                    }
-                }
-                spb::fence_proxy_async();
-                __syncwarp();
-                if (lane == 0) arrive(spb::smem_u32(&sm.q_full[i]));
+                for (int c = 0; c < HD / 32; c++)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + 512 * c),
+                                 "l"(bytes ? q + 32 * c : static_cast<const T *>(a.q)), "r"(bytes) : "memory");
             }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            __syncwarp();
+            {
+                unsigned char *mine = own + (lane >> 3) * (HD * 16) + (lane & 7) * 16;
+#pragma unroll 4
+                for (int c = 0; c < HD / 8; c++) {
+                    const uint4 x = *reinterpret_cast<const uint4 *>(mine + 128 * c);
+#pragma unroll
+                    for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(sp_load_as_float(reinterpret_cast<const T *>(&x), j)));
+                }
+                float down, up;
+                row_scale(top, down, up);
+                mul = fabsf(a.scale) * kLog2e * up;
+                if (a.scale < 0.0f) down = -down;
+#pragma unroll 2
+                for (int c = 0; c < HD / 8; c++) {
+                    const uint4 x = *reinterpret_cast<const uint4 *>(mine + 128 * c);
+                    __half h[8];
+#pragma unroll
+                    for (int j = 0; j < 8; j++)
+                        h[j] = __float2half_rn(sp_load_as_float(reinterpret_cast<const T *>(&x), j) * down);
+                    *reinterpret_cast<uint4 *>(mine + 128 * c) = *reinterpret_cast<const uint4 *>(h);
+                }
+            }
+            spb::fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) arrive(spb::smem_u32(&sm.q_full[i]));
             const int hi = !real ? 0x7fffffff : a.causal ? pos : w.e.kv_len - 1;
             const int lo = real && a.window > 0 ? pos - a.window + 1 : 0;
             const long long slot = (long long)w.e.seq * a.l.heads + w.head;
@@ -432,123 +457,175 @@ __global__ void __launch_bounds__(Shape<HD>::Threads, 1) k_q8_attn_many(const __
                 const uint32_t t_s = tmem + lanes + (NQ == 2 ? 128 : 64) * buf;
                 if (!wait(sm.s_full[buf], NQ == 2 ? done : done >> 1)) goto out;
                 fence_after();
-                uint32_t p[BN / 2];
-                float sum = 0.0f, over = 0.0f;
-                // ---- weights relative to the maximum so far; over: the largest exponent
-                auto weights = [&](auto masked) {
-                    uint32_t v[2][16];
-                    tmem_ld16(t_s, v[0]);
-                    sum = 0.0f;
-                    over = -INFINITY;
-#pragma unroll
-                    for (int c = 0; c < BN / 16; c++) {
-                        const float fg = __shfl_sync(0xffffffffu, f, c) * mul;
-                        const float off = __shfl_sync(0xffffffffu, lv, c) - m, ig = __shfl_sync(0xffffffffu, iv, c);
-                        wait_ld();
-                        if (c + 1 < BN / 16) tmem_ld16(t_s + 16 * (c + 1), v[(c + 1) & 1]);
-                        const uint32_t(&u)[16] = v[c & 1];
-                        F2 part = {0.0f, 0.0f};
-#pragma unroll
-                        for (int j = 0; j < 16; j += 2) {
-                            F2 x = fma2({__uint_as_float(u[j]), __uint_as_float(u[j + 1])}, {fg, fg}, {off, off});
-                            if (decltype(masked)::value) {
-                                const int at = j0 + 16 * c + j;
-                                if (at > hi || at < lo) x.x = -INFINITY;
-                                if (at + 1 > hi || at + 1 < lo) x.y = -INFINITY;
-                            }
-                            over = max3(over, x.x, x.y);
-                            x.x = ex2(x.x);
-                            x.y = ex2(x.y);
-                            part = add2(part, x);
-                            const __half2 hw = __floats2half2_rn(x.x, x.y);
-                            p[8 * c + j / 2] = *reinterpret_cast<const uint32_t *>(&hw);
-                        }
-                        sum = fmaf(part.x + part.y, ig, sum);
-                    }
-                };
-                // ---- a row's first tile, and one whose scores pass the maximum by more
-                // than 2^8: the maximum is found before the weights are taken
-                auto raise = [&]() {
+                // A larger maximum, of positions 32 c .. 32 c + 31 too: what the products so
+                // far have summed, and this tile's weights before them, shrink.
+                auto raise = [&](int c, bool masked) {
                     float top = kNone;
 #pragma unroll 1
-                    for (int c = 0; c < BN / 16; c++) {
-                        const float fg = __shfl_sync(0xffffffffu, f, c) * mul, lg = __shfl_sync(0xffffffffu, lv, c);
+                    for (int h = 2 * c; h < 2 * c + 2; h++) {
+                        const float fg = __shfl_sync(0xffffffffu, f, h) * mul, lg = __shfl_sync(0xffffffffu, lv, h);
                         uint32_t v[16];
-                        tmem_ld16(t_s + 16 * c, v);
-                        wait_ld();
+                        tmem_ld16(t_s + 16 * h, v);
+                        wait_ld16(v);
 #pragma unroll
                         for (int j = 0; j < 16; j++) {
-                            const int at = j0 + 16 * c + j;
-                            if (at <= hi && at >= lo) top = fmaxf(top, fmaf(__uint_as_float(v[j]), fg, lg));
+                            const int at = j0 + 16 * h + j;
+                            if (!masked || (at <= hi && at >= lo)) top = fmaxf(top, fmaf(__uint_as_float(v[j]), fg, lg));
                         }
                     }
-                    const bool up = top > m + 8.0f;
+                    const bool up = top > m + 4.0f;         // a sum over 2^12 has a weight over 2^8
                     const float fix = up ? ex2(m - top) : 1.0f;
                     if (up) m = top;
                     l *= fix;
-                    if (k == k0) return true;
-                    // the products so far are in: the values that they summed shrink too
-                    if (!wait(sm.pv_done[i], done - 1)) return false;
-                    fence_after();
+                    if (k > k0) {
+                        if (!wait_values(done - 1)) return false;
+                        fence_after();
 #pragma unroll 1
-                    for (int c = 0; c < HD; c += 16) {
-                        uint32_t v[16];
-                        tmem_ld16(t_o + c, v);
-                        wait_ld();
+                        for (int d = 0; d < HD; d += 16) {
+                            uint32_t v[16];
+                            tmem_ld16(t_o + d, v);
+                            wait_ld16(v);
 #pragma unroll
-                        for (int j = 0; j < 16; j++) v[j] = __float_as_uint(__uint_as_float(v[j]) * fix);
-                        tmem_st16(t_o + c, v);
+                            for (int j = 0; j < 16; j++) v[j] = __float_as_uint(__uint_as_float(v[j]) * fix);
+                            tmem_st16(t_o + d, v);
+                        }
                     }
                     wait_st();
+                    const __half2 x = __float2half2_rn(fix);
+#pragma unroll 1
+                    for (int d = 0; d < 16 * c; d += 16) {
+                        uint32_t v[16];
+                        tmem_ld16(t_s + d, v);
+                        wait_ld16(v);
+#pragma unroll
+                        for (int j = 0; j < 16; j++) {
+                            const __half2 y = __hmul2(*reinterpret_cast<const __half2 *>(&v[j]), x);
+                            v[j] = *reinterpret_cast<const uint32_t *>(&y);
+                        }
+                        tmem_st16(t_s + d, v);
+                    }
                     return true;
                 };
-                bool fresh = k == k0;
-                for (;;) {
-                    if (fresh && !raise()) goto out;
-                    if (all) weights(std::false_type{});
-                    else weights(std::true_type{});
-                    if (fresh || !__any_sync(0xffffffffu, over > 8.0f)) break;
-                    fresh = true;
-                }
-                l += sum;
-                if constexpr (BN == 128) {
-                    tmem_st32(t_s, reinterpret_cast<const uint32_t(&)[32]>(p[0]));
-                    tmem_st32(t_s + 32, reinterpret_cast<const uint32_t(&)[32]>(p[32]));
-                } else {
-                    tmem_st32(t_s, reinterpret_cast<const uint32_t(&)[32]>(p[0]));
-                }
+                // ---- 32 positions at a time: weights by the maximum so far; where 16 of
+                // them sum up to more than 2^12 the maximum is raised and they are taken
+                // again (no weight passes 2^12 otherwise, well inside fp16)
+                auto weights = [&](auto masked) {
+                    constexpr bool kMasked = decltype(masked)::value;
+                    uint32_t u[32];
+                    tmem_ld32(t_s, u);
+                    // the scales of 32 positions, fetched a step ahead: a shuffle waits
+                    // behind the exponentials in flight
+                    float fn[2], ln[2], in[2];
+                    auto scales_of = [&](int c) {
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            fn[h] = __shfl_sync(0xffffffffu, f, 2 * c + h);
+                            ln[h] = __shfl_sync(0xffffffffu, lv, 2 * c + h);
+                            in[h] = __shfl_sync(0xffffffffu, iv, 2 * c + h);
+                        }
+                    };
+                    scales_of(0);
+                    // not unrolled: the instruction cache is what several roles at once
+                    // are short of
+#pragma unroll 1
+                    for (int c = 0; c < BN / 32; c++) {
+                        uint32_t p[16];
+                        float sum;
+                        const float fc[2] = {fn[0], fn[1]}, lc[2] = {ln[0], ln[1]}, ic[2] = {in[0], in[1]};
+                        wait_ld32(u);
+#pragma unroll 1
+                        for (int again = 0;; again = 1) {
+                            F2 x[16];
+                            float fg[2], off[2];
+#pragma unroll
+                            for (int h = 0; h < 2; h++) {
+                                fg[h] = fc[h] * mul;
+                                off[h] = lc[h] - m;
+                            }
+#pragma unroll
+                            for (int j = 0; j < 16; j++) {
+                                x[j] = fma2({__uint_as_float(u[2 * j]), __uint_as_float(u[2 * j + 1])}, {fg[j / 8], fg[j / 8]}, {off[j / 8], off[j / 8]});
+                                if (kMasked) {
+                                    const int at = j0 + 32 * c + 2 * j;
+                                    if (at > hi || at < lo) x[j].x = -INFINITY;
+                                    if (at + 1 > hi || at + 1 < lo) x[j].y = -INFINITY;
+                                }
+                            }
+                            if (c + 1 < BN / 32) tmem_ld32(t_s + 32 * (c + 1), u);
+                            scales_of(c + 1);
+                            bool over = false;
+                            sum = 0.0f;
+#pragma unroll
+                            for (int h = 0; h < 2; h++) {
+                                F2 part = {0.0f, 0.0f};
+#pragma unroll
+                                for (int j = 8 * h; j < 8 * h + 8; j++) {
+                                    if (!kMasked && kPoly(j)) {
+                                        x[j] = exp2_poly(x[j]);
+                                    } else {
+                                        x[j].x = ex2(x[j].x);
+                                        x[j].y = ex2(x[j].y);
+                                    }
+                                    part = add2(part, x[j]);
+                                    const __half2 hw = __floats2half2_rn(x[j].x, x[j].y);
+                                    p[j] = *reinterpret_cast<const uint32_t *>(&hw);
+                                }
+                                over |= part.x + part.y > 4096.0f;
+                                sum = fmaf(part.x + part.y, ic[h], sum);
+                            }
+                            // once: exponents past 2^26 no longer differ from the maximum by
+                            // less than their own rounding
+                            if (again || !__any_sync(0xffffffffu, over)) break;
+                            if (!raise(c, kMasked)) return false;
+                            tmem_ld32(t_s + 32 * c, u);
+                            wait_ld32(u);
+                        }
+                        l += sum;
+                        tmem_st16(t_s + 16 * c, p);
+                    }
+                    return true;
+                };
+                if (!(all ? weights(std::false_type{}) : weights(std::true_type{}))) goto out;
                 wait_st();
                 fence_before();
                 __syncwarp();
                 if (lane == 0) arrive(spb::smem_u32(&sm.p_full[buf]));
             }
-            // ---- the unit's result, or this run's part of it.  With two buffers of
-            // scores this warp may be two products ahead: a phase is waited for
-            // only after the one before it.
-            if (NQ == 1 && k1 - k0 > 1 && !wait(sm.pv_done[i], done - 2)) goto out;
-            if (!wait(sm.pv_done[i], done - 1)) goto out;
+            // ---- the unit's result, or this run's part of it
+            if (!wait_values(done - 1)) goto out;
             fence_after();
             const bool whole = k0 == 0 && k1 == w.r.tiles;
-            constexpr float kOut = 1.0f / Unit<FMT>::v;
             if (whole) {
-                const float inv = l > 0.0f ? kOut / l : 0.0f;
-                T *out = static_cast<T *>(a.out) + (long long)tok * a.out_stride + qh * HD;
+                const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+                // through the warp's own part of the queries' place, so that a row's
+                // bytes leave together: 16-byte pieces, exchanged within groups of
+                // eight by the row to fall on different banks
 #pragma unroll 1
                 for (int c = 0; c < HD; c += 32) {
                     uint32_t v[32];
                     tmem_ld32(t_o + c, v);
-                    wait_ld();
-                    if (real) {
+                    wait_ld32(v);
 #pragma unroll
-                        for (int b = 0; b < 32; b += 8) {
-                            T x[8];
+                    for (int b = 0; b < 32; b += 8) {
+                        T x[8];
 #pragma unroll
-                            for (int j = 0; j < 8; j++)
-                                x[j] = T(__uint_as_float(v[b + (j & 4) + ((j & 3) >> 1) + 2 * (j & 1)]) * inv);
-                            *reinterpret_cast<uint4 *>(out + c + b) = *reinterpret_cast<const uint4 *>(x);
-                        }
+                        for (int j = 0; j < 8; j++)
+                            x[j] = T(__uint_as_float(v[b + j]) * inv);
+                        *reinterpret_cast<uint4 *>(own + lane * HD * 2 + (((c + b) / 8) ^ (lane & 7)) * 16) = *reinterpret_cast<const uint4 *>(x);
                     }
                 }
+                __syncwarp();
+                constexpr int kPieces = HD / 8;                  // of a row
+#pragma unroll 4
+                for (int n = lane; n < 32 * kPieces; n += 32) {
+                    const int rr = n / kPieces, pc = n % kPieces, ar = w.r.row0 + 128 * i + 32 * (warp & 3) + rr;
+                    if (ar < w.r.row0 + w.r.rows) {
+                        T *out = static_cast<T *>(a.out) + (long long)(w.e.q0 + ar / a.group) * a.out_stride +
+                                 (w.head * a.group + ar % a.group) * HD;
+                        reinterpret_cast<uint4 *>(out)[pc] = *reinterpret_cast<const uint4 *>(own + rr * HD * 2 + (pc ^ (rr & 7)) * 16);
+                    }
+                }
+                __syncwarp();
                 if (real && a.lse) a.lse[(long long)tok * a.n_q_heads + qh] = l > 0.0f ? kLn2 * (m + lg2(l)) : -INFINITY;
             } else {
                 // rows side by side, so that a warp's stores are contiguous
@@ -558,12 +635,12 @@ __global__ void __launch_bounds__(Shape<HD>::Threads, 1) k_q8_attn_many(const __
                 for (int c = 0; c < HD; c += 32) {
                     uint32_t v[32];
                     tmem_ld32(t_o + c, v);
-                    wait_ld();
+                    wait_ld32(v);
                     if (real) {
 #pragma unroll
                         for (int b = 0; b < 32; b += 4)
                             __stcg(reinterpret_cast<float4 *>(part) + (c + b) / 4 * S::ROWS + prow,
-                                   make_float4(__uint_as_float(v[b]), __uint_as_float(v[b + 2]), __uint_as_float(v[b + 1]),
+                                   make_float4(__uint_as_float(v[b]), __uint_as_float(v[b + 1]), __uint_as_float(v[b + 2]),
                                                __uint_as_float(v[b + 3])));
                     }
                 }
@@ -580,21 +657,24 @@ __global__ void __launch_bounds__(Shape<HD>::Threads, 1) k_q8_attn_many(const __
         // 16 codes a lane at a time: 8 positions x 4 runs of 16 dimensions, so
         // that eight lanes' 16-byte stores fill a core matrix
         const int cw = warp - S::SoftWarps;
-        constexpr int kLoads = BN * HD / 16 / (32 * S::ConvWarps);
         constexpr int kSpan = HD / 64;                           // 64-dimension spans of a row
+        constexpr int kUnits = BN / 8 * kSpan;                   // (8 positions, 64 dimensions)
+        constexpr int kLoads = (kUnits + S::ConvWarps - 1) / S::ConvWarps;
         unsigned done = 0;
         uint4 kx[kLoads], vx[kLoads];                            // each loaded a tile ahead
         auto load = [&](uint4(&x)[kLoads], const uint8_t *p) {
 #pragma unroll
             for (int n = 0; n < kLoads; n++) {
-                const int u = cw + S::ConvWarps * n;             // (8 positions, 64 dimensions)
-                x[n] = *reinterpret_cast<const uint4 *>(p + (long long)(u / kSpan * 8 + (lane & 7)) * HD + u % kSpan * 64 + (lane >> 3) * 16);
+                const int u = cw + S::ConvWarps * n;
+                if (u < kUnits)
+                    x[n] = *reinterpret_cast<const uint4 *>(p + (long long)(u / kSpan * 8 + (lane & 7)) * HD + u % kSpan * 64 + (lane >> 3) * 16);
             }
         };
         auto store = [&](const uint4(&x)[kLoads], unsigned char *dst, unsigned long long &full) {
 #pragma unroll
             for (int n = 0; n < kLoads; n++) {
                 const int u = cw + S::ConvWarps * n;
+                if (u >= kUnits) break;
                 unsigned char *d = dst + (u / kSpan) * (HD * 16) + (u % kSpan * 8 + (lane >> 3) * 2) * 128 + (lane & 7) * 16;
                 uint4 lo, hi;
                 unpack4<FMT>(x[n].x, lo.x, lo.y);
@@ -615,18 +695,27 @@ __global__ void __launch_bounds__(Shape<HD>::Threads, 1) k_q8_attn_many(const __
             const int k0 = w.k0(), k1 = w.k1();
             load(kx, kp + (long long)k0 * BN * HD);
             load(vx, vp + (long long)k0 * BN * HD);
+            // codes of V past the end may be NaN, which a weight of 0 does not undo
+            auto no_nan = [&](int j0) {
+                if (FMT == SP_Q8_E4M3 && j0 + BN > w.e.kv_len) {
+#pragma unroll
+                    for (int n = 0; n < kLoads; n++)
+                        if (j0 + (cw + S::ConvWarps * n) / kSpan * 8 + (lane & 7) >= w.e.kv_len) vx[n] = make_uint4(0u, 0u, 0u, 0u);
+                }
+            };
             for (int k = k0; k < k1; k++, done++) {
                 const int st = done & 1;
                 if (done >= 2 && !wait(sm.k_free[st], done / 2 - 1)) goto out;
                 store(kx, sm.k[st], sm.k_full[st]);
                 if (k + 1 < k1) load(kx, kp + (long long)(k + 1) * BN * HD);
                 if (done >= 2 && !wait(sm.v_free[st], done / 2 - 1)) goto out;
+                no_nan(w.r.start + k * BN);
                 store(vx, sm.v[st], sm.v_full[st]);
                 if (k + 1 < k1) load(vx, vp + (long long)(k + 1) * BN * HD);
             }
         }
-    } else if (warp == kMmaWarp && lane == 0) {
-        // ================= the tensor cores' thread =================
+    } else if (warp == kMmaWarp) {
+        // ================= the tensor cores' warp =================
         unsigned done = 0, units = 0;
         auto scores = [&](int i, unsigned n) {                   // tile n of the run, counted over all units
             const uint32_t q = spb::smem_u32(sm.q[i]), k = spb::smem_u32(sm.k[n & 1]);
@@ -642,27 +731,27 @@ __global__ void __launch_bounds__(Shape<HD>::Threads, 1) k_q8_attn_many(const __
 #pragma unroll
             for (int s = 0; s < BN / 16; s++)
                 mma_ts(tmem + S::ColO + HD * i, p + 8 * s, operand(v + s * 2 * (HD * 16), HD * 16, 128), instr(HD, true), add || s > 0);
-            commit(spb::smem_u32(&sm.pv_done[i]));
+            commit(spb::smem_u32(&sm.pv_done[NQ == 2 ? i : n & 1]));
         };
         for (; w.more(); w.next(a), units++) {
             const int n = w.k1() - w.k0();
-            if (!wait1(sm.k_full[done & 1], done / 2)) goto mma_out;
+            if (!wait(sm.k_full[done & 1], done / 2)) goto mma_out;
             for (int i = 0; i < NQ; i++) {
-                if (!wait1(sm.q_full[i], units)) goto mma_out;
+                if (!wait(sm.q_full[i], units)) goto mma_out;
                 fence_after();
                 scores(i, done);
             }
             commit(spb::smem_u32(&sm.k_free[done & 1]));
             for (int k = 0; k < n; k++, done++) {
-                if (k + 1 < n && !wait1(sm.k_full[(done + 1) & 1], (done + 1) / 2)) goto mma_out;
+                if (k + 1 < n && !wait(sm.k_full[(done + 1) & 1], (done + 1) / 2)) goto mma_out;
                 if (NQ == 1 && k + 1 < n) {
                     fence_after();
                     scores(0, done + 1);
                     commit(spb::smem_u32(&sm.k_free[(done + 1) & 1]));
                 }
                 for (int i = 0; i < NQ; i++) {
-                    if (i == 0 && !wait1(sm.v_full[done & 1], done / 2)) goto mma_out;
-                    if (!wait1(sm.p_full[NQ == 2 ? i : done & 1], NQ == 2 ? done : done >> 1)) goto mma_out;
+                    if (i == 0 && !wait(sm.v_full[done & 1], done / 2)) goto mma_out;
+                    if (!wait(sm.p_full[NQ == 2 ? i : done & 1], NQ == 2 ? done : done >> 1)) goto mma_out;
                     fence_after();
                     values(i, done, k > 0);
                     if (NQ == 2 && k + 1 < n) scores(i, done + 1);
@@ -674,7 +763,7 @@ __global__ void __launch_bounds__(Shape<HD>::Threads, 1) k_q8_attn_many(const __
     mma_out:
         // whatever was issued is over before tensor memory goes back
         commit(spb::smem_u32(&sm.end));
-        spb::wait_stage(spb::smem_u32(&sm.end), 0, nullptr);
+        if (lane == 0) spb::wait_stage(spb::smem_u32(&sm.end), 0, nullptr);
     }
 out:
     __syncwarp();
@@ -714,7 +803,7 @@ __global__ void __launch_bounds__(Shape<HD>::ROWS) k_q8_attn_join(const __grid_c
             acc[4 * j + 3] = fmaf(x[j].w, f1, acc[4 * j + 3] * f0);
         }
     }
-    const float inv = sum > 0.0f ? (1.0f / Unit<FMT>::v) / sum : 0.0f;
+    const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
     const int rr = sp.row0 + row, tok = sp.q0 + rr / a.group, qh = sp.head * a.group + rr % a.group;
     T x[16];
 #pragma unroll
