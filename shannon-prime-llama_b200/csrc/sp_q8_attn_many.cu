@@ -31,7 +31,12 @@ struct Shape {
     static constexpr int SoftWarps = 4 * NQ, ConvWarps = 15 - SoftWarps;
     static constexpr int Threads = 32 * (SoftWarps + ConvWarps + 1);   // the last warp issues the products
     static constexpr int ColO = 256;                   // S (and P) at 128 i or 64 (k & 1), O at 256 + HD i
-    static constexpr int StageB = BN * HD * 2, QB = 128 * HD * 2;
+    // Operands lie in core matrices of 8 rows of 16 bytes, the next 8 dimensions'
+    // Core bytes on: 16 more than a core matrix has, so that the stores of 4
+    // lanes for each row, whose loads are then 64 contiguous bytes, fall on
+    // different banks.  Products run at the same rate as without the gap.
+    static constexpr int Core = 144, Rows8 = HD / 8 * Core;
+    static constexpr int StageB = BN / 8 * Rows8, QB = 16 * Rows8;
     static constexpr int SlotFloats = ROWS * (HD + 2);
 };
 
@@ -40,6 +45,7 @@ struct ManySmem {
     unsigned char q[Shape<HD>::NQ][Shape<HD>::QB];
     unsigned char k[2][Shape<HD>::StageB], v[2][Shape<HD>::StageB];
     unsigned long long q_full[2], k_full[2], k_free[2], v_full[2], v_free[2], s_full[2], p_full[2], pv_done[2], end;
+    float4 scales[Shape<HD>::SoftWarps][Shape<HD>::BN / 16];   // of a tile: K scale, log2 of V's, 1 / V's
     unsigned scan[32];
     unsigned tiles[256];                               // of one head of each entry of a chunk, then their prefix
     int found;
@@ -135,9 +141,8 @@ __device__ __forceinline__ F2 exp2_poly(F2 x)
 }
 
 // Shared-memory operand without swizzle, in core matrices of 8 rows of 16
-// bytes: byte offsets between core matrices along and across the leading
-// direction (K-major: lbo along K, sbo along M or N; MN-major: lbo along K,
-// sbo along M or N too).
+// bytes: lbo bytes between core matrices along K, sbo along M or N (for both
+// the K-major and the MN-major operands).
 __device__ __forceinline__ uint64_t operand(uint32_t addr, uint32_t lbo, uint32_t sbo)
 {
     return (uint64_t)((addr & 0x3FFFFu) >> 4) | (uint64_t)((lbo >> 4) & 0x3FFFu) << 16 |
@@ -392,25 +397,25 @@ __global__ void __launch_bounds__(Shape<HD>::Threads, 1) k_q8_attn_many(const __
             // time, into the operand's places as they are; then a thread for each
             // row scales its own to fp16
             float mul, top = 0.0f;
-            unsigned char *own = sm.q[i] + (warp & 3) * 4 * (HD * 16);
+            unsigned char *own = sm.q[i] + (warp & 3) * 4 * S::Rows8;
 #pragma unroll 1
             for (int n = 0; n < 4; n++) {
-                const int rr = 128 * i + 32 * (warp & 3) + 8 * n + (lane & 7), ar = w.r.row0 + rr;
+                const int rr = 128 * i + 32 * (warp & 3) + 8 * n + (lane >> 2), ar = w.r.row0 + rr;
                 const T *q = static_cast<const T *>(a.q) + (long long)(w.e.q0 + ar / a.group) * a.q_stride +
-                             (w.head * a.group + ar % a.group) * HD + (lane >> 3) * 8;
-                const uint32_t dst = spb::smem_u32(own + n * (HD * 16) + lane * 16), bytes = rr < w.r.rows ? 16 : 0;
+                             (w.head * a.group + ar % a.group) * HD + (lane & 3) * 8;
+                const uint32_t dst = spb::smem_u32(own + n * S::Rows8 + (lane & 3) * S::Core + (lane >> 2) * 16), bytes = rr < w.r.rows ? 16 : 0;
 #pragma unroll
                 for (int c = 0; c < HD / 32; c++)
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + 512 * c),
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + 4 * S::Core * c),
                                  "l"(bytes ? q + 32 * c : static_cast<const T *>(a.q)), "r"(bytes) : "memory");
             }
             asm volatile("cp.async.wait_all;" ::: "memory");
             __syncwarp();
             {
-                unsigned char *mine = own + (lane >> 3) * (HD * 16) + (lane & 7) * 16;
+                unsigned char *mine = own + (lane >> 3) * S::Rows8 + (lane & 7) * 16;
 #pragma unroll 4
                 for (int c = 0; c < HD / 8; c++) {
-                    const uint4 x = *reinterpret_cast<const uint4 *>(mine + 128 * c);
+                    const uint4 x = *reinterpret_cast<const uint4 *>(mine + S::Core * c);
 #pragma unroll
                     for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(sp_load_as_float(reinterpret_cast<const T *>(&x), j)));
                 }
@@ -420,12 +425,12 @@ __global__ void __launch_bounds__(Shape<HD>::Threads, 1) k_q8_attn_many(const __
                 if (a.scale < 0.0f) down = -down;
 #pragma unroll 2
                 for (int c = 0; c < HD / 8; c++) {
-                    const uint4 x = *reinterpret_cast<const uint4 *>(mine + 128 * c);
+                    const uint4 x = *reinterpret_cast<const uint4 *>(mine + S::Core * c);
                     __half h[8];
 #pragma unroll
                     for (int j = 0; j < 8; j++)
                         h[j] = __float2half_rn(sp_load_as_float(reinterpret_cast<const T *>(&x), j) * down);
-                    *reinterpret_cast<uint4 *>(mine + 128 * c) = *reinterpret_cast<const uint4 *>(h);
+                    *reinterpret_cast<uint4 *>(mine + S::Core * c) = *reinterpret_cast<const uint4 *>(h);
                 }
             }
             spb::fence_proxy_async();
@@ -439,7 +444,9 @@ __global__ void __launch_bounds__(Shape<HD>::Threads, 1) k_q8_attn_many(const __
             float m = kNone, l = 0.0f;
             const int k0 = w.k0(), k1 = w.k1();
             // a lane for each 16 positions of a tile: their scales, loaded a tile
-            // ahead (harmless ones past the end)
+            // ahead (harmless ones past the end) and passed to the others through
+            // shared memory (as shuffles, three for each 16 positions, they cost a
+            // quarter of the loop)
             float ks = 0.0f, vs = 1.0f;
             auto load_scales = [&](int k) {
                 const int at = w.r.start + k * BN + 16 * (lane % (BN / 16));
@@ -450,7 +457,9 @@ __global__ void __launch_bounds__(Shape<HD>::Threads, 1) k_q8_attn_many(const __
             load_scales(k0);
             for (int k = k0; k < k1; k++, done++) {
                 const int j0 = w.r.start + k * BN;
-                const float vc = fmaxf(vs, kScaleMin), lv = lg2(vc), iv = __frcp_rn(vc), f = ks;
+                const float vc = fmaxf(vs, kScaleMin);
+                if (lane < BN / 16) sm.scales[warp][lane] = make_float4(ks, lg2(vc), __frcp_rn(vc), 0.0f);
+                __syncwarp();
                 if (k + 1 < k1) load_scales(k + 1);
                 const bool all = __all_sync(0xffffffffu, j0 + BN - 1 <= hi && j0 >= lo);
                 const int buf = NQ == 2 ? i : (int)(done & 1);
@@ -463,7 +472,8 @@ __global__ void __launch_bounds__(Shape<HD>::Threads, 1) k_q8_attn_many(const __
                     float top = kNone;
 #pragma unroll 1
                     for (int h = 2 * c; h < 2 * c + 2; h++) {
-                        const float fg = __shfl_sync(0xffffffffu, f, h) * mul, lg = __shfl_sync(0xffffffffu, lv, h);
+                        const float4 sc = sm.scales[warp][h];
+                        const float fg = sc.x * mul, lg = sc.y;
                         uint32_t v[16];
                         tmem_ld16(t_s + 16 * h, v);
                         wait_ld16(v);
@@ -513,25 +523,16 @@ __global__ void __launch_bounds__(Shape<HD>::Threads, 1) k_q8_attn_many(const __
                     constexpr bool kMasked = decltype(masked)::value;
                     uint32_t u[32];
                     tmem_ld32(t_s, u);
-                    // the scales of 32 positions, fetched a step ahead: a shuffle waits
-                    // behind the exponentials in flight
-                    float fn[2], ln[2], in[2];
-                    auto scales_of = [&](int c) {
-#pragma unroll
-                        for (int h = 0; h < 2; h++) {
-                            fn[h] = __shfl_sync(0xffffffffu, f, 2 * c + h);
-                            ln[h] = __shfl_sync(0xffffffffu, lv, 2 * c + h);
-                            in[h] = __shfl_sync(0xffffffffu, iv, 2 * c + h);
-                        }
-                    };
-                    scales_of(0);
+                    // the scales of 32 positions, read a step ahead
+                    const float4 *sc = sm.scales[warp];
+                    float4 next[2] = {sc[0], sc[1]};
                     // not unrolled: the instruction cache is what several roles at once
                     // are short of
 #pragma unroll 1
                     for (int c = 0; c < BN / 32; c++) {
                         uint32_t p[16];
                         float sum;
-                        const float fc[2] = {fn[0], fn[1]}, lc[2] = {ln[0], ln[1]}, ic[2] = {in[0], in[1]};
+                        const float4 now[2] = {next[0], next[1]};
                         wait_ld32(u);
 #pragma unroll 1
                         for (int again = 0;; again = 1) {
@@ -539,8 +540,8 @@ __global__ void __launch_bounds__(Shape<HD>::Threads, 1) k_q8_attn_many(const __
                             float fg[2], off[2];
 #pragma unroll
                             for (int h = 0; h < 2; h++) {
-                                fg[h] = fc[h] * mul;
-                                off[h] = lc[h] - m;
+                                fg[h] = now[h].x * mul;
+                                off[h] = now[h].y - m;
                             }
 #pragma unroll
                             for (int j = 0; j < 16; j++) {
@@ -552,7 +553,7 @@ __global__ void __launch_bounds__(Shape<HD>::Threads, 1) k_q8_attn_many(const __
                                 }
                             }
                             if (c + 1 < BN / 32) tmem_ld32(t_s + 32 * (c + 1), u);
-                            scales_of(c + 1);
+                            if (c + 1 < BN / 32) next[0] = sc[2 * c + 2], next[1] = sc[2 * c + 3];
                             bool over = false;
                             sum = 0.0f;
 #pragma unroll
@@ -571,7 +572,7 @@ __global__ void __launch_bounds__(Shape<HD>::Threads, 1) k_q8_attn_many(const __
                                     p[j] = *reinterpret_cast<const uint32_t *>(&hw);
                                 }
                                 over |= part.x + part.y > 4096.0f;
-                                sum = fmaf(part.x + part.y, ic[h], sum);
+                                sum = fmaf(part.x + part.y, now[h].z, sum);
                             }
                             // once: exponents past 2^26 no longer differ from the maximum by
                             // less than their own rounding
@@ -654,8 +655,8 @@ __global__ void __launch_bounds__(Shape<HD>::Threads, 1) k_q8_attn_many(const __
         }
     } else if (warp < S::SoftWarps + S::ConvWarps) {
         // ================= codes to fp16 operands =================
-        // 16 codes a lane at a time: 8 positions x 4 runs of 16 dimensions, so
-        // that eight lanes' 16-byte stores fill a core matrix
+        // 16 codes a lane at a time, 8 positions x 4 runs of 16 dimensions, four
+        // lanes for a position
         const int cw = warp - S::SoftWarps;
         constexpr int kSpan = HD / 64;                           // 64-dimension spans of a row
         constexpr int kUnits = BN / 8 * kSpan;                   // (8 positions, 64 dimensions)
@@ -667,7 +668,7 @@ __global__ void __launch_bounds__(Shape<HD>::Threads, 1) k_q8_attn_many(const __
             for (int n = 0; n < kLoads; n++) {
                 const int u = cw + S::ConvWarps * n;
                 if (u < kUnits)
-                    x[n] = *reinterpret_cast<const uint4 *>(p + (long long)(u / kSpan * 8 + (lane & 7)) * HD + u % kSpan * 64 + (lane >> 3) * 16);
+                    x[n] = *reinterpret_cast<const uint4 *>(p + (long long)(u / kSpan * 8 + (lane >> 2)) * HD + u % kSpan * 64 + (lane & 3) * 16);
             }
         };
         auto store = [&](const uint4(&x)[kLoads], unsigned char *dst, unsigned long long &full) {
@@ -675,14 +676,14 @@ __global__ void __launch_bounds__(Shape<HD>::Threads, 1) k_q8_attn_many(const __
             for (int n = 0; n < kLoads; n++) {
                 const int u = cw + S::ConvWarps * n;
                 if (u >= kUnits) break;
-                unsigned char *d = dst + (u / kSpan) * (HD * 16) + (u % kSpan * 8 + (lane >> 3) * 2) * 128 + (lane & 7) * 16;
+                unsigned char *d = dst + u / kSpan * S::Rows8 + (u % kSpan * 8 + (lane & 3) * 2) * S::Core + (lane >> 2) * 16;
                 uint4 lo, hi;
                 unpack4<FMT>(x[n].x, lo.x, lo.y);
                 unpack4<FMT>(x[n].y, lo.z, lo.w);
                 unpack4<FMT>(x[n].z, hi.x, hi.y);
                 unpack4<FMT>(x[n].w, hi.z, hi.w);
                 *reinterpret_cast<uint4 *>(d) = lo;
-                *reinterpret_cast<uint4 *>(d + 128) = hi;
+                *reinterpret_cast<uint4 *>(d + S::Core) = hi;
             }
             spb::fence_proxy_async();
             __syncwarp();
@@ -700,18 +701,21 @@ __global__ void __launch_bounds__(Shape<HD>::Threads, 1) k_q8_attn_many(const __
                 if (FMT == SP_Q8_E4M3 && j0 + BN > w.e.kv_len) {
 #pragma unroll
                     for (int n = 0; n < kLoads; n++)
-                        if (j0 + (cw + S::ConvWarps * n) / kSpan * 8 + (lane & 7) >= w.e.kv_len) vx[n] = make_uint4(0u, 0u, 0u, 0u);
+                        if (j0 + (cw + S::ConvWarps * n) / kSpan * 8 + (lane >> 2) >= w.e.kv_len) vx[n] = make_uint4(0u, 0u, 0u, 0u);
                 }
             };
             for (int k = k0; k < k1; k++, done++) {
                 const int st = done & 1;
                 if (done >= 2 && !wait(sm.k_free[st], done / 2 - 1)) goto out;
                 store(kx, sm.k[st], sm.k_full[st]);
-                if (k + 1 < k1) load(kx, kp + (long long)(k + 1) * BN * HD);
                 if (done >= 2 && !wait(sm.v_free[st], done / 2 - 1)) goto out;
                 no_nan(w.r.start + k * BN);
                 store(vx, sm.v[st], sm.v_full[st]);
-                if (k + 1 < k1) load(vx, vp + (long long)(k + 1) * BN * HD);
+                // both after the last fence: a fence waits for loads in flight too
+                if (k + 1 < k1) {
+                    load(kx, kp + (long long)(k + 1) * BN * HD);
+                    load(vx, vp + (long long)(k + 1) * BN * HD);
+                }
             }
         }
     } else if (warp == kMmaWarp) {
@@ -722,7 +726,7 @@ __global__ void __launch_bounds__(Shape<HD>::Threads, 1) k_q8_attn_many(const __
             const uint32_t d = tmem + (NQ == 2 ? 128 * i : 64 * (n & 1));
 #pragma unroll
             for (int s = 0; s < HD / 16; s++)
-                mma_ss(d, operand(q + s * 256, 128, HD * 16), operand(k + s * 256, 128, HD * 16), instr(BN, false), s > 0);
+                mma_ss(d, operand(q + 2 * s * S::Core, S::Core, S::Rows8), operand(k + 2 * s * S::Core, S::Core, S::Rows8), instr(BN, false), s > 0);
             commit(spb::smem_u32(&sm.s_full[NQ == 2 ? i : n & 1]));
         };
         auto values = [&](int i, unsigned n, bool add) {
@@ -730,7 +734,7 @@ __global__ void __launch_bounds__(Shape<HD>::Threads, 1) k_q8_attn_many(const __
             const uint32_t p = tmem + (NQ == 2 ? 128 * i : 64 * (n & 1));
 #pragma unroll
             for (int s = 0; s < BN / 16; s++)
-                mma_ts(tmem + S::ColO + HD * i, p + 8 * s, operand(v + s * 2 * (HD * 16), HD * 16, 128), instr(HD, true), add || s > 0);
+                mma_ts(tmem + S::ColO + HD * i, p + 8 * s, operand(v + 2 * s * S::Rows8, S::Rows8, S::Core), instr(HD, true), add || s > 0);
             commit(spb::smem_u32(&sm.pv_done[NQ == 2 ? i : n & 1]));
         };
         for (; w.more(); w.next(a), units++) {
