@@ -13,18 +13,15 @@ using namespace q8;
 constexpr int kWarps = 8, kThreads = 32 * kWarps;
 constexpr int kTile = 16 * kWarps;       // positions of a tile: 16 for each warp
 
-__device__ __forceinline__ uint4 ldg16(const uint8_t *p)
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t dst, const uint8_t *src)
 {
-    uint4 v;
-    asm("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-    return v;
+    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ uint2 ldg8(const uint8_t *p)
-{
-    uint2 v;
-    asm("ld.global.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
-    return v;
-}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
 {
@@ -55,8 +52,17 @@ __device__ __forceinline__ Unit0 unit_of(const AttnArgs &a, const Entry &e)
     return u;
 }
 
-template <int HD, int NT>
+// A warp's stage: 16 rows of K and of V as they are in memory, rows a little
+// apart so that the fragments' reads fall on different banks.
+template <int HD>
+struct Stage {
+    static constexpr int KPitch = HD + 16, VPitch = HD + 16;
+    static constexpr int Bytes = 16 * (KPitch + VPitch);
+};
+
+template <int HD, int NT, int STAGES>
 struct FewSmem {
+    unsigned char ring[kWarps][STAGES][Stage<HD>::Bytes];
     uint2 q[NT][HD / 16][32];                 // query fragments, one 8-byte word a lane
     float up[8 * NT];                         // 2^exponent of each row
     float m[kWarps][8 * NT], l[kWarps][8 * NT];
@@ -81,14 +87,14 @@ struct FewSmem {
 // rounded to fp16 for the product alone, relative to what they contribute,
 // and the sum of the unscaled weights is kept beside them in 32 bits as
 // sum w / vs.
-template <typename T, int FMT, int HD, int NT, int CTAS>
+template <typename T, int FMT, int HD, int NT, int STAGES, int CTAS>
 __global__ void __launch_bounds__(kThreads, CTAS) k_q8_attn_few(const __grid_constant__ AttnArgs a)
 {
     constexpr int KS = HD / 16;               // k-steps of the scores, 32-bit code words of a K row in a lane
     constexpr int VW = HD / 32;               // code words of a V row in a lane
     constexpr bool kQInRegs = NT * KS <= 8;
     extern __shared__ __align__(16) unsigned char smem_raw[];
-    FewSmem<HD, NT> &sm = *reinterpret_cast<FewSmem<HD, NT> *>(smem_raw);
+    FewSmem<HD, NT, STAGES> &sm = *reinterpret_cast<FewSmem<HD, NT, STAGES> *>(smem_raw);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
     const int H = a.l.heads, G = a.group;
 
@@ -156,50 +162,40 @@ __global__ void __launch_bounds__(kThreads, CTAS) k_q8_attn_few(const __grid_con
         const float *ksp = a.l.k_scale + slot * (a.l.max_seq >> a.l.block_log2);
         const float *vsp = a.l.v_scale + slot * (a.l.max_seq >> a.l.block_log2);
 
-        uint32_t kw[2][KS], vw[4][VW];
-        float ks = 0.0f, vs = 1.0f;
-        auto load_k = [&](int j0) {
+        // ---- the warp's ring: 16 positions a stage, copied a few stages ahead
+        using St = Stage<HD>;
+        const uint32_t ring = (uint32_t)__cvta_generic_to_shared(sm.ring[warp]);
+        auto fetch = [&](int j0, int st) {
+            constexpr int kChunks = HD / 16, kRows = 32 / kChunks;       // 16-byte pieces of a row, rows at a time
+            const int r0 = lane / kChunks, pc = lane % kChunks * 16;
+            const uint32_t dk = ring + st * St::Bytes + r0 * St::KPitch + pc, dv = dk + 16 * St::KPitch;
+            const long long at = (long long)(j0 + r0) * HD + pc;
 #pragma unroll
-            for (int r = 0; r < 2; r++)
-#pragma unroll
-                for (int j = 0; j < KS / 4; j++) {
-                    const uint4 w = ldg16(kp + (long long)(j0 + g + 8 * r) * HD + 64 * j + 16 * c);
-                    kw[r][4 * j] = w.x; kw[r][4 * j + 1] = w.y; kw[r][4 * j + 2] = w.z; kw[r][4 * j + 3] = w.w;
-                }
-            ks = ksp[j0 >> a.l.block_log2];
-        };
-        auto load_v = [&](int j0) {
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const uint8_t *p = vp + (long long)(j0 + 2 * c + (r & 1) + 8 * (r >> 1)) * HD;
-                if constexpr (HD == 64) {
-                    const uint2 w = ldg8(p + 8 * g);
-                    vw[r][0] = w.x; vw[r][1] = w.y;
-                } else {
-#pragma unroll
-                    for (int i = 0; i < HD / 128; i++) {
-                        const uint4 w = ldg16(p + 128 * i + 16 * g);
-                        vw[r][4 * i] = w.x; vw[r][4 * i + 1] = w.y; vw[r][4 * i + 2] = w.z; vw[r][4 * i + 3] = w.w;
-                    }
-                }
+            for (int r = 0; r < 16; r += kRows) {
+                copy_async<16>(dk + r * St::KPitch, kp + at + r * HD);
+                copy_async<16>(dv + r * St::VPitch, vp + at + r * HD);
             }
-            // codes past the end may be NaN, which a weight of 0 does not undo
-            if (FMT == SP_Q8_E4M3 && j0 + 15 >= e.kv_len) {
-#pragma unroll
-                for (int r = 0; r < 4; r++)
-                    if (j0 + 2 * c + (r & 1) + 8 * (r >> 1) >= e.kv_len) {
-#pragma unroll
-                        for (int i = 0; i < VW; i++) vw[r][i] = 0;
-                    }
-            }
-            vs = vsp[j0 >> a.l.block_log2];
         };
         // dimension of code word i of a V row
         auto dim_of = [&](int i) { return HD == 64 ? 8 * g + 4 * i : 128 * (i / 4) + 16 * g + 4 * (i % 4); };
 
         int j0 = u.start + k0 * kTile + 16 * warp;
         const int j_stop = min(u.end, u.start + k1 * kTile);
-        if (j0 < j_stop) { load_k(j0); load_v(j0); }
+        int jf = j0;                           // next positions to fetch
+        float ks[STAGES], vs[STAGES];          // scales of the stages in flight, oldest first
+#pragma unroll
+        for (int i = 0; i < STAGES; i++) {
+            ks[i] = 0.0f;
+            vs[i] = 1.0f;
+            if (jf < j_stop) {
+                fetch(jf, i);
+                ks[i] = ksp[jf >> a.l.block_log2];
+                vs[i] = vsp[jf >> a.l.block_log2];
+            }
+            copy_commit();
+            jf += kTile;
+        }
+        int st = 0;
 
         // ---- queries: scaled to fp16, in fragment order
 #pragma unroll
@@ -262,6 +258,9 @@ __global__ void __launch_bounds__(kThreads, CTAS) k_q8_attn_few(const __grid_con
                 for (int j = 0; j < 4; j++) o[n][i][j] = 0.0f;
 
         for (; j0 < j_stop; j0 += kTile) {
+            copy_wait<STAGES - 1>();
+            __syncwarp();
+            const unsigned char *stage = sm.ring[warp][st];
             // ---- scores of 16 positions
             float s[NT][4];
 #pragma unroll
@@ -269,19 +268,33 @@ __global__ void __launch_bounds__(kThreads, CTAS) k_q8_attn_few(const __grid_con
 #pragma unroll
                 for (int j = 0; j < 4; j++) s[n][j] = 0.0f;
 #pragma unroll
-            for (int i = 0; i < KS; i++) {
-                uint32_t f[4];
-                unpack4<FMT>(kw[0][i], f[0], f[2]);
-                unpack4<FMT>(kw[1][i], f[1], f[3]);
+            for (int q = 0; q < KS / 4; q++) {
+                uint4 w[2];
 #pragma unroll
-                for (int n = 0; n < NT; n++) {
-                    const uint2 b = kQInRegs ? qr[kQInRegs ? n : 0][kQInRegs ? i : 0] : sm.q[n][i][lane];
-                    mma(s[n], f, b.x, b.y);
+                for (int r = 0; r < 2; r++) w[r] = *reinterpret_cast<const uint4 *>(stage + (g + 8 * r) * St::KPitch + 64 * q + 16 * c);
+#pragma unroll
+                for (int x = 0; x < 4; x++) {
+                    const int i = 4 * q + x;
+                    uint32_t f[4];
+                    unpack4<FMT>(reinterpret_cast<const uint32_t *>(&w[0])[x], f[0], f[2]);
+                    unpack4<FMT>(reinterpret_cast<const uint32_t *>(&w[1])[x], f[1], f[3]);
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        const uint2 b = kQInRegs ? qr[kQInRegs ? n : 0][kQInRegs ? i : 0] : sm.q[n][i][lane];
+                        mma(s[n], f, b.x, b.y);
+                    }
                 }
             }
-            const float k_scale = ks, v_scale = fmaxf(vs, kScaleMin);
-            const int next = j0 + kTile;
-            if (next < j_stop) load_k(next);
+            const float k_scale = ks[0], v_scale = fmaxf(vs[0], kScaleMin);
+#pragma unroll
+            for (int i = 0; i + 1 < STAGES; i++) {
+                ks[i] = ks[i + 1];
+                vs[i] = vs[i + 1];
+            }
+            if (jf < j_stop) {
+                ks[STAGES - 1] = ksp[jf >> a.l.block_log2];
+                vs[STAGES - 1] = vsp[jf >> a.l.block_log2];
+            }
 
             // ---- weights
             const float lv = lg2(v_scale), iv = __frcp_rn(v_scale);
@@ -336,19 +349,43 @@ __global__ void __launch_bounds__(kThreads, CTAS) k_q8_attn_few(const __grid_con
                 }
             }
             // ---- values
+            {
+                constexpr int kWide = HD == 64 ? 2 : 4;        // code words of a lane's run of a row
+                const unsigned char *vst = stage + 16 * St::KPitch + 2 * c * St::VPitch + 4 * kWide * g;
 #pragma unroll
-            for (int i = 0; i < VW; i++) {
+                for (int q = 0; q < VW / kWide; q++) {
+                    uint32_t w[4][kWide];
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    uint32_t f[4];
-                    const unsigned pick = h ? 0x7362 : 0x5140;     // a dimension of two positions side by side
-                    unpack4<FMT>(__byte_perm(vw[0][i], vw[1][i], pick), f[0], f[1]);
-                    unpack4<FMT>(__byte_perm(vw[2][i], vw[3][i], pick), f[2], f[3]);
+                    for (int r = 0; r < 4; r++) {
+                        const unsigned char *p8 = vst + ((r & 1) + 8 * (r >> 1)) * St::VPitch + 128 * q;
+                        if constexpr (kWide == 2) *reinterpret_cast<uint2 *>(w[r]) = *reinterpret_cast<const uint2 *>(p8);
+                        else *reinterpret_cast<uint4 *>(w[r]) = *reinterpret_cast<const uint4 *>(p8);
+                        // codes past the end may be NaN, which a weight of 0 does not undo
+                        if (FMT == SP_Q8_E4M3 && j0 + 15 >= e.kv_len && j0 + 2 * c + (r & 1) + 8 * (r >> 1) >= e.kv_len) {
 #pragma unroll
-                    for (int n = 0; n < NT; n++) mma(o[n][2 * i + h], f, p[n][0], p[n][1]);
+                            for (int x = 0; x < kWide; x++) w[r][x] = 0;
+                        }
+                    }
+#pragma unroll
+                    for (int x = 0; x < kWide; x++) {
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            const int i = kWide * q + x;
+                            uint32_t f[4];
+                            const unsigned pick = h ? 0x7362 : 0x5140;     // a dimension of two positions side by side
+                            unpack4<FMT>(__byte_perm(w[0][x], w[1][x], pick), f[0], f[1]);
+                            unpack4<FMT>(__byte_perm(w[2][x], w[3][x], pick), f[2], f[3]);
+#pragma unroll
+                            for (int n = 0; n < NT; n++) mma(o[n][2 * i + h], f, p[n][0], p[n][1]);
+                        }
+                    }
                 }
             }
-            if (next < j_stop) load_v(next);
+            __syncwarp();                      // all lanes have read the stage
+            if (jf < j_stop) fetch(jf, st);
+            copy_commit();
+            jf += kTile;
+            st = st + 1 == STAGES ? 0 : st + 1;
         }
 
         // ---- the warps' results into one: rows lie in shared memory in the
@@ -488,10 +525,12 @@ __global__ void __launch_bounds__(kThreads, CTAS) k_q8_attn_few(const __grid_con
 template <typename T, int FMT, int HD, int NT>
 int launch_few(const AttnArgs &a, int sms, unsigned tiles, cudaStream_t s)
 {
-    // CTAs on an SM: what the registers of 256 threads allow without spilling
+    // CTAs on an SM: what the registers of 256 threads allow without spilling;
+    // stages: what shared memory then holds
     constexpr int CTAS = NT * HD <= 64 ? 3 : NT * HD <= 128 ? 2 : 1;
-    auto kernel = k_q8_attn_few<T, FMT, HD, NT, CTAS>;
-    constexpr int smem = sizeof(FewSmem<HD, NT>);
+    constexpr int STAGES = HD == 64 ? (NT == 1 ? 3 : 4) : HD == 128 ? (NT == 1 ? 2 : 3) : 2;
+    auto kernel = k_q8_attn_few<T, FMT, HD, NT, STAGES, CTAS>;
+    constexpr int smem = sizeof(FewSmem<HD, NT, STAGES>);
     static std::atomic<unsigned long long> ready{0};      // devices whose attribute is set
     int dev = 0;
     cudaGetDevice(&dev);
