@@ -235,17 +235,25 @@ __global__ void __launch_bounds__(kThreads, CTAS) k_q8_attn_few(const __grid_con
                 for (int s = 0; s < KS; s++) qr[n][s] = sm.q[n][s][lane];
         }
         float mul[NT][2], m[NT][2], l[NT][2];
-        int hi[NT][2], lo[NT][2];
+        // the positions that a row sees: kept with 8 rows, found again where a mask
+        // asks for them with more, whose registers then hold two CTAs on an SM
+        int hi[2], lo[2];
+        auto limits = [&](int n, int i, int &h, int &w) {
+            const int pos = first + (8 * n + 2 * c + i) / G;
+            h = a.causal ? pos : e.kv_len - 1;
+            w = a.window > 0 ? pos - a.window + 1 : 0;
+        };
+        if (NT == 1) {
+            limits(0, 0, hi[0], lo[0]);
+            limits(0, 1, hi[1], lo[1]);
+        }
         const int hi_min = a.causal ? first : e.kv_len - 1;
         const int lo_max = a.window > 0 ? e.kv_len - a.window : 0;
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                const int row = 8 * n + 2 * c + i, pos = first + row / G;
-                mul[n][i] = a.scale * kLog2e * sm.up[row];
-                hi[n][i] = a.causal ? pos : e.kv_len - 1;
-                lo[n][i] = a.window > 0 ? pos - a.window + 1 : 0;
+                mul[n][i] = a.scale * kLog2e * sm.up[8 * n + 2 * c + i];
                 m[n][i] = kNone;
                 l[n][i] = 0.0f;
             }
@@ -309,8 +317,9 @@ __global__ void __launch_bounds__(kThreads, CTAS) k_q8_attn_few(const __grid_con
                     s[n][2 + i] = fmaf(s[n][2 + i], f, lv);
                     if (!all) {
                         const int j = j0 + g;
-                        if (j > hi[n][i] || j < lo[n][i]) s[n][i] = -INFINITY;
-                        if (j + 8 > hi[n][i] || j + 8 < lo[n][i]) s[n][2 + i] = -INFINITY;
+                        if (NT > 1) limits(n, i, hi[i], lo[i]);
+                        if (j > hi[i] || j < lo[i]) s[n][i] = -INFINITY;
+                        if (j + 8 > hi[i] || j + 8 < lo[i]) s[n][2 + i] = -INFINITY;
                     }
                     over |= fmaxf(s[n][i], s[n][2 + i]) > m[n][i] + 8.0f;
                 }
@@ -527,8 +536,8 @@ int launch_few(const AttnArgs &a, int sms, unsigned tiles, cudaStream_t s)
 {
     // CTAs on an SM: what the registers of 256 threads allow without spilling;
     // stages: what shared memory then holds
-    constexpr int CTAS = NT * HD <= 64 ? 3 : NT * HD <= 128 ? 2 : 1;
-    constexpr int STAGES = HD == 64 ? (NT == 1 ? 3 : 4) : HD == 128 ? (NT == 1 ? 2 : 3) : 2;
+    constexpr int CTAS = HD == 256 || NT * HD == 512 ? 1 : NT * HD <= 64 ? 3 : 2;
+    constexpr int STAGES = HD == 256 || (HD == 64 && NT == 4) || (HD == 128 && NT < 4) ? 2 : 3;
     auto kernel = k_q8_attn_few<T, FMT, HD, NT, STAGES, CTAS>;
     constexpr int smem = sizeof(FewSmem<HD, NT, STAGES>);
     static std::atomic<unsigned long long> ready{0};      // devices whose attribute is set
