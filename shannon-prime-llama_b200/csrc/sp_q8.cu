@@ -41,7 +41,8 @@ extern "C" int sp_cuda_q8_cache_init(sp_cuda_q8_cache_t *qc, const sp_config_t *
     sp_clear_error();
     if (!qc || !cfg) return sp_set_error(SP_ERR_ARG, "q8_cache_init: NULL argument");
     memset(qc, 0, sizeof(*qc));
-    if (cfg->n_layers <= 0 || cfg->n_heads_kv <= 0 || n_seqs <= 0 || max_seq_len <= 0 || max_seq_len > (1 << 30))
+    if (cfg->n_layers <= 0 || cfg->n_heads_kv <= 0 || cfg->n_heads_kv > 32767 || n_seqs <= 0 || max_seq_len <= 0 ||
+        max_seq_len > (1 << 30))
         return sp_set_error(SP_ERR_ARG, "q8_cache_init: bad dims");
     if (cfg->head_dim != 64 && cfg->head_dim != 128 && cfg->head_dim != 256)
         return sp_set_error(SP_ERR_UNSUPPORTED, "q8_cache_init: head_dim %d is not 64, 128 or 256", cfg->head_dim);
@@ -125,6 +126,7 @@ struct WriteArgs {
     q8::Batch b;
     long long token_stride;    // elements
     int heads, max_seq, block_log2;
+    int slots, slots_each;     // (half, head) pairs of a block, and how many of them a CTA takes in turn
 };
 
 template <typename T>
@@ -138,18 +140,67 @@ __device__ __forceinline__ float raw_at(const Raw8<T> &r, int i)
     return sp_load_as_float(reinterpret_cast<const T *>(r.w), i);
 }
 
-// Codes of 8 values already in units of the scale.
-template <int FMT>
-__device__ __forceinline__ uint2 encode8(const float (&x)[8])
+// The largest magnitude of 8 inputs and `top`; NaN if any is NaN.
+__device__ __forceinline__ float max_nan(float a, float b)
+{
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+template <typename T>
+struct Top;
+template <>
+struct Top<float> {
+    float v = 0.0f;
+    __device__ __forceinline__ void add(const Raw8<float> &r)
+    {
+#pragma unroll
+        for (int i = 0; i < 8; i++) v = max_nan(v, fabsf(raw_at(r, i)));
+    }
+    __device__ __forceinline__ float value() const { return v; }
+};
+template <>
+struct Top<__half> {
+    __half2 v = __float2half2_rn(0.0f);
+    __device__ __forceinline__ void add(const Raw8<__half> &r)
+    {
+        const __half2 *x = reinterpret_cast<const __half2 *>(r.w);
+#pragma unroll
+        for (int i = 0; i < 4; i++) v = __hmax2_nan(v, __habs2(x[i]));
+    }
+    __device__ __forceinline__ float value() const { return max_nan(__low2float(v), __high2float(v)); }
+};
+template <>
+struct Top<__nv_bfloat16> {
+    __nv_bfloat162 v = __float2bfloat162_rn(0.0f);
+    __device__ __forceinline__ void add(const Raw8<__nv_bfloat16> &r)
+    {
+        const __nv_bfloat162 *x = reinterpret_cast<const __nv_bfloat162 *>(r.w);
+#pragma unroll
+        for (int i = 0; i < 4; i++) v = __hmax2_nan(v, __habs2(x[i]));
+    }
+    __device__ __forceinline__ float value() const { return max_nan(__low2float(v), __high2float(v)); }
+};
+
+// Codes of 8 values already in units of the scale; CHECKED: they may be NaN or
+// pass the largest code by more than rounding.
+template <int FMT, bool CHECKED>
+__device__ __forceinline__ uint2 encode8(float (&x)[8])
 {
     uint2 r;
+    if (CHECKED) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = x[i] == x[i] ? x[i] : 0.0f;
+    }
     if constexpr (FMT == SP_Q8_INT8) {
         // adding 1.5 * 2^23 rounds to a whole number, ties to even, which then
         // stands in the low bits
         uint32_t q[8];
 #pragma unroll
-        for (int i = 0; i < 8; i++)
-            q[i] = __float_as_uint(__fadd_rn(fmaxf(fminf(x[i], 127.0f), -127.0f), 12582912.0f));
+        for (int i = 0; i < 8; i++) {
+            if (CHECKED) x[i] = fmaxf(fminf(x[i], 127.0f), -127.0f);
+            q[i] = __float_as_uint(__fadd_rn(x[i], 12582912.0f));
+        }
         r.x = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
         r.y = __byte_perm(__byte_perm(q[4], q[5], 0x0040), __byte_perm(q[6], q[7], 0x0040), 0x5410);
     } else {
@@ -163,19 +214,21 @@ __device__ __forceinline__ uint2 encode8(const float (&x)[8])
     return r;
 }
 
-// One CTA for one block of one sequence, head and half; block * HD / 32
-// threads, each with four groups of 8 adjacent elements, so the block's input
-// is read once and stays in registers while its maximum is found.
-template <typename T, int FMT, int HD>
-__global__ void __launch_bounds__(1024) k_q8_write(const __grid_constant__ WriteArgs a)
+// One CTA for one block of one sequence, and in it one (half, head) pair after
+// another; block * HD / 32 threads, each with four groups of 8 adjacent
+// elements, so the input is read once and stays in registers while the CTA
+// finds its maximum.  The next pair's input is on its way meanwhile.  (A cluster
+// of CTAs of 256 threads for the larger blocks, joining their maxima through
+// shared memory, took 1.4 times as long.)
+template <typename T, int FMT, int HD, int THREADS>
+__global__ void __launch_bounds__(THREADS) k_q8_write(const __grid_constant__ WriteArgs a)
 {
     constexpr int kPerToken = HD / 8;
-    const WriteHalf &h = a.h[blockIdx.y];
-    const int unit = blockIdx.x / a.heads, head = blockIdx.x - unit * a.heads;
-    const int B = 1 << a.block_log2;
+    constexpr bool kAhead = sizeof(T) == 2 || THREADS < 1024;   // 1024 threads have 64 registers
+    const int unit = blockIdx.x;
 
     // which sequence and block: a running sum of the blocks that each entry touches
-    const int lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     int blk = -1, before = 0;
     q8::Entry e = {0, 0, 0, 0};
     for (int base = 0; base < a.b.n_seqs && blk < 0; base += 32) {
@@ -210,72 +263,128 @@ __global__ void __launch_bounds__(1024) k_q8_write(const __grid_constant__ Write
     if (blk < 0) return;                         // the grid is an upper bound
 
     const int p0 = e.kv_len - e.n, lo = blk << a.block_log2;
-    const long long slot = (long long)e.seq * a.heads + head;
-    uint8_t *codes = h.codes + (slot * a.max_seq + lo) * HD;
-    float *scale = h.scale + slot * (a.max_seq >> a.block_log2) + blk;
     const bool keeps = p0 > lo;                  // older positions stay in this block
-    const float old = keeps ? *scale : 0.0f;
+    const int s0 = blockIdx.y * a.slots_each, s1 = min(s0 + a.slots_each, a.slots);
+    __shared__ float tops[2][THREADS / 32];
 
-    Raw8<T> raw[4];
-    float top = 0.0f;
+    auto load = [&](Raw8<T>(&raw)[4], int slot) {
+        const int half = slot / a.heads, head = slot - half * a.heads;
 #pragma unroll
-    for (int c = 0; c < 4; c++) {
-        const int g = c * blockDim.x + threadIdx.x;
-        const int pos = lo + g / kPerToken;
-        if (pos >= p0 && pos < e.kv_len) {
-            const T *src = static_cast<const T *>(h.in) + (long long)(e.q0 + pos - p0) * a.token_stride + head * HD +
-                           (g % kPerToken) * 8;
+        for (int c = 0; c < 4; c++) {
+            const int g = c * blockDim.x + threadIdx.x;
+            const int pos = lo + g / kPerToken;
+            if (pos >= p0 && pos < e.kv_len) {
+                const T *src = static_cast<const T *>(a.h[half].in) + (long long)(e.q0 + pos - p0) * a.token_stride +
+                               head * HD + (g % kPerToken) * 8;
 #pragma unroll
-            for (int i = 0; i < (int)sizeof(T) / 2; i++) raw[c].w[i] = reinterpret_cast<const uint4 *>(src)[i];
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const float m = fabsf(raw_at(raw[c], i));
-                if (m <= 3.402823466e38f) top = fmaxf(top, m);    // neither infinity nor NaN
+                for (int i = 0; i < (int)sizeof(T) / 2; i++) raw[c].w[i] = __ldcs(reinterpret_cast<const uint4 *>(src) + i);
             }
+        }
+    };
+    auto one = [&](const Raw8<T>(&raw)[4], Raw8<T>(&next)[4], int slot) {
+        const int half = slot / a.heads, head = slot - half * a.heads, odd = slot & 1;
+        const WriteHalf &h = a.h[half];
+        const long long at = (long long)e.seq * a.heads + head;
+        uint8_t *codes = h.codes + (at * a.max_seq + lo) * HD;
+        float *scale = h.scale + at * (a.max_seq >> a.block_log2) + blk;
+        const float old = keeps ? *scale : 0.0f;
+        if (kAhead && slot + 1 < s1) load(next, slot + 1);
+        Top<T> most;
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            const int pos = lo + (c * (int)blockDim.x + (int)threadIdx.x) / kPerToken;
+            if (pos >= p0 && pos < e.kv_len) most.add(raw[c]);
+        }
+        // a thread with an infinity or NaN says so by a negative maximum of the others
+        float top = most.value();
+        if (!(top <= 3.402823466e38f)) {
+            top = 0.0f;
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                const int pos = lo + (c * (int)blockDim.x + (int)threadIdx.x) / kPerToken;
+                if (pos >= p0 && pos < e.kv_len) {
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const float m = fabsf(raw_at(raw[c], i));
+                        if (m <= 3.402823466e38f) top = fmaxf(top, m);
+                    }
+                }
+            }
+            top = -top;
+        }
+        bool odd_values = __any_sync(0xffffffffu, __float_as_uint(top) >> 31);
+        top = fabsf(top);
+#pragma unroll
+        for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        if (lane == 0) tops[odd][warp] = odd_values ? -top : top;
+        __syncthreads();
+        top = 0.0f;
+        odd_values = false;
+        for (int i = 0; i < warps; i++) {
+            odd_values |= __float_as_uint(tops[odd][i]) >> 31;
+            top = fmaxf(top, fabsf(tops[odd][i]));
+        }
+
+        float s = fminf(fmaxf(__fmul_rn(top, 1.0f / q8::code_max(FMT)), q8::kScaleMin), q8::kScaleMax);
+        const bool grown = keeps && s > old;
+        s = fmaxf(s, old);
+        const float inv = __frcp_rn(s);
+        // values this CTA has that are NaN or out of the codes' range
+        const bool checked = odd_values || !(top * inv < q8::code_max(FMT) + 0.25f);
+        if (threadIdx.x == 0) *scale = s;            // all have read the old one: the barrier above
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            const int g = c * blockDim.x + threadIdx.x;
+            const int pos = lo + g / kPerToken;
+            uint2 *dst = reinterpret_cast<uint2 *>(codes + (long long)g * 8);
+            float x[8];
+            if (pos >= p0 && pos < e.kv_len) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) x[i] = __fmul_rn(raw_at(raw[c], i), inv);
+                *dst = checked ? encode8<FMT, true>(x) : encode8<FMT, false>(x);
+            } else if (grown && pos < p0) {
+                const float ratio = __fdiv_rn(old, s);
+                const uint2 w = *dst;
+                const uint8_t *b = reinterpret_cast<const uint8_t *>(&w);
+#pragma unroll
+                for (int i = 0; i < 8; i++) x[i] = __fmul_rn(q8::decode1<FMT>(b[i]), ratio);
+                *dst = encode8<FMT, true>(x);
+            }
+        }
+    };
+    Raw8<T> x[4], y[4];
+    if (kAhead) {
+        load(x, s0);
+        for (int slot = s0; slot < s1; slot += 2) {
+            one(x, y, slot);
+            if (slot + 1 < s1) one(y, x, slot + 1);
+        }
+    } else {
+        for (int slot = s0; slot < s1; slot++) {
+            load(x, slot);
+            one(x, x, slot);
         }
     }
-    __shared__ float tops[32];
-#pragma unroll
-    for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-    if (lane == 0) tops[threadIdx.x >> 5] = top;
-    __syncthreads();
-    top = 0.0f;
-    for (int i = 0; i < (int)(blockDim.x >> 5); i++) top = fmaxf(top, tops[i]);
+}
 
-    float s = fminf(fmaxf(__fmul_rn(top, 1.0f / q8::code_max(FMT)), q8::kScaleMin), q8::kScaleMax);
-    const bool grown = keeps && s > old;
-    s = fmaxf(s, old);
-    const float inv = __frcp_rn(s), ratio = __fdiv_rn(old, s);
-    if (threadIdx.x == 0) *scale = s;            // all have read the old one: the barrier above
-#pragma unroll
-    for (int c = 0; c < 4; c++) {
-        const int g = c * blockDim.x + threadIdx.x;
-        const int pos = lo + g / kPerToken;
-        uint2 *dst = reinterpret_cast<uint2 *>(codes + (long long)g * 8);
-        float x[8];
-        if (pos >= p0 && pos < e.kv_len) {
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const float v = __fmul_rn(raw_at(raw[c], i), inv);
-                x[i] = v == v ? v : 0.0f;
-            }
-            *dst = encode8<FMT>(x);
-        } else if (grown && pos < p0) {
-            const uint2 w = *dst;
-            const uint8_t *b = reinterpret_cast<const uint8_t *>(&w);
-#pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = __fmul_rn(q8::decode1<FMT>(b[i]), ratio);
-            *dst = encode8<FMT>(x);
-        }
+template <typename T, int FMT, int HD>
+void launch_write_hd(const WriteArgs &a, dim3 grid, int threads, cudaStream_t s)
+{
+    if (threads <= 256) k_q8_write<T, FMT, HD, 256><<<grid, threads, 0, s>>>(a);
+    if constexpr (HD >= 128) {
+        if (threads == 512) k_q8_write<T, FMT, HD, 512><<<grid, threads, 0, s>>>(a);
+    }
+    if constexpr (HD == 256) {
+        if (threads == 1024) k_q8_write<T, FMT, HD, 1024><<<grid, threads, 0, s>>>(a);
     }
 }
 
 template <typename T, int FMT>
 void launch_write(const WriteArgs &a, int hd, dim3 grid, int threads, cudaStream_t s)
 {
-    if (hd == 64) k_q8_write<T, FMT, 64><<<grid, threads, 0, s>>>(a);
-    else if (hd == 128) k_q8_write<T, FMT, 128><<<grid, threads, 0, s>>>(a);
-    else k_q8_write<T, FMT, 256><<<grid, threads, 0, s>>>(a);
+    if (hd == 64) launch_write_hd<T, FMT, 64>(a, grid, threads, s);
+    else if (hd == 128) launch_write_hd<T, FMT, 128>(a, grid, threads, s);
+    else launch_write_hd<T, FMT, 256>(a, grid, threads, s);
 }
 
 template <int FMT>
@@ -319,9 +428,15 @@ extern "C" int sp_cuda_q8_write_kv_tokens(sp_cuda_q8_cache_t *qc, int layer, con
     const long long B = qc->block_tokens;
     const long long each = batch->n_seqs * ((batch->max_new + B - 2) / B + 1);
     const long long all = batch->n_tokens / B + 2ll * batch->n_seqs;
-    const long long units = (each < all ? each : all) * H;
-    if (units > 0x7fffffff) return sp_set_error(SP_ERR_ARG, "q8_write: %lld blocks in one call", units);
-    const dim3 grid((unsigned)units, n);
+    const long long units = each < all ? each : all;
+    if (units > 0x7fffffff / 4) return sp_set_error(SP_ERR_ARG, "q8_write: %lld blocks in one call", units);
+    a.slots = n * H;
+    // Pairs in turn where there are blocks enough to fill the SMs several times
+    // over: a step of single tokens wants a CTA for each instead.
+    long long in_turn = units * a.slots / (16ll * qc->sm_count);
+    in_turn = in_turn < 1 ? 1 : in_turn > 16 ? 16 : in_turn;
+    a.slots_each = (int)(in_turn < a.slots ? in_turn : a.slots);
+    const dim3 grid((unsigned)units, (a.slots + a.slots_each - 1) / a.slots_each);
     const int threads = (int)(B * hd / 32);
     cudaStream_t s = (cudaStream_t)qc->stream;
     if (qc->format == SP_Q8_INT8) launch_write_of<SP_Q8_INT8>(a, dtype, hd, grid, threads, s);
@@ -333,49 +448,87 @@ extern "C" int sp_cuda_q8_write_kv_tokens(sp_cuda_q8_cache_t *qc, int layer, con
 
 namespace {
 
-constexpr int kReadThreads = 256;
+constexpr int kReadThreads = 256, kReadUnits = 4;
 
-// Each thread turns four codes into four values; a warp's loads and stores
-// are contiguous.
-template <typename T, int FMT>
-__global__ void __launch_bounds__(kReadThreads)
-k_q8_read(const uint8_t *codes, const float *scale, int heads, int max_seq, int hd_log2, int block_log2, int start,
-          long long n, T *out)
+struct ReadArgs {
+    const uint8_t *codes;          // of the sequence's first head
+    const float *scale;
+    void *out;
+    int heads, max_seq, hd_log2, block_log2, start;
+    unsigned n;                    // units of a head
+};
+
+// The values of 8 codes (4 of them where x.y is not given).
+template <int FMT, int E>
+__device__ __forceinline__ void decode8(uint2 c, float (&x)[8])
 {
-    for (long long i = (long long)blockIdx.x * kReadThreads + threadIdx.x; i < n; i += (long long)gridDim.x * kReadThreads) {
-        const long long el = i * 4, row = el >> hd_log2;
-        const int d = (int)(el - (row << hd_log2));
-        const int t = (int)(row / heads), head = (int)(row - (long long)t * heads);
-        const int pos = start + t;
-        const uchar4 c = *reinterpret_cast<const uchar4 *>(codes + ((((long long)head * max_seq + pos) << hd_log2) + d));
-        const float s = scale[(long long)head * (max_seq >> block_log2) + (pos >> block_log2)];
-        const float x[4] = {q8::decode1<FMT>(c.x) * s, q8::decode1<FMT>(c.y) * s, q8::decode1<FMT>(c.z) * s,
-                            q8::decode1<FMT>(c.w) * s};
-        if constexpr (sizeof(T) == 4) {
-            *reinterpret_cast<float4 *>(out + el) = make_float4(x[0], x[1], x[2], x[3]);
-        } else {
-            uint2 w;
-            T *e = reinterpret_cast<T *>(&w);
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                if constexpr (sizeof(T) == 2) e[j] = T(x[j]);
-            }
-            *reinterpret_cast<uint2 *>(out + el) = w;
+    for (int w = 0; w < E / 4; w++) {
+        const uint32_t v = w ? c.y : c.x;
+        if constexpr (FMT == SP_Q8_INT8) {
+            // q + 128 in the low bits of 2^23
+            const uint32_t u = v ^ 0x80808080u;
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                x[4 * w + i] = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7540 + i)) - 8388736.0f;
+        } else {
+            uint32_t a, b;
+            asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+                : "=r"(a), "=r"(b) : "r"(v));
+            const float2 p = __half22float2(*reinterpret_cast<const __half2 *>(&a)), q = __half22float2(*reinterpret_cast<const __half2 *>(&b));
+            x[4 * w] = p.x; x[4 * w + 1] = p.y; x[4 * w + 2] = q.x; x[4 * w + 3] = q.y;
+        }
+    }
+}
+
+// A row of CTAs for each head.  Each thread turns kReadUnits units of codes (16
+// bytes of values each) into values; a warp's loads and stores of one unit are
+// contiguous within a position.
+template <typename T, int FMT>
+__global__ void __launch_bounds__(kReadThreads) k_q8_read(const __grid_constant__ ReadArgs a)
+{
+    constexpr int E = 16 / sizeof(T);              // codes of a unit
+    const int unit_log2 = a.hd_log2 - (E == 8 ? 3 : 2);
+    const int head = blockIdx.y;
+    const uint8_t *codes = a.codes + (((long long)head * a.max_seq + a.start) << a.hd_log2);
+    const float *scale = a.scale + (long long)head * (a.max_seq >> a.block_log2);
+    char *out = (char *)a.out + ((long long)head << a.hd_log2) * sizeof(T);
+    const long long row_bytes = ((long long)a.heads << a.hd_log2) * sizeof(T);
+    uint2 c[kReadUnits];
+    float s[kReadUnits];
+    const unsigned u0 = blockIdx.x * (kReadThreads * kReadUnits) + threadIdx.x;
+#pragma unroll
+    for (int k = 0; k < kReadUnits; k++) {
+        const unsigned u = u0 + k * kReadThreads;
+        if (u < a.n) {
+            if constexpr (E == 8) c[k] = __ldcs(reinterpret_cast<const uint2 *>(codes) + u);
+            else c[k].x = __ldcs(reinterpret_cast<const unsigned *>(codes) + u);
+            s[k] = scale[(a.start + (u >> unit_log2)) >> a.block_log2];
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < kReadUnits; k++) {
+        const unsigned u = u0 + k * kReadThreads;
+        if (u < a.n) {
+            float v[8];
+            decode8<FMT, E>(c[k], v);
+            uint4 w;
+            T *x = reinterpret_cast<T *>(&w);
+#pragma unroll
+            for (int i = 0; i < E; i++) x[i] = T(v[i] * s[k]);
+            const unsigned t = u >> unit_log2;
+            __stcs(reinterpret_cast<uint4 *>(out + t * row_bytes) + (u - (t << unit_log2)), w);
         }
     }
 }
 
 template <int FMT>
-void launch_read(const uint8_t *codes, const float *scale, int heads, int max_seq, int hd_log2, int block_log2, int start,
-                 long long n, void *out, int dtype, unsigned grid, cudaStream_t s)
+void launch_read(const ReadArgs &a, int dtype, cudaStream_t s)
 {
-    if (dtype == SP_DTYPE_F32)
-        k_q8_read<float, FMT><<<grid, kReadThreads, 0, s>>>(codes, scale, heads, max_seq, hd_log2, block_log2, start, n, (float *)out);
-    else if (dtype == SP_DTYPE_F16)
-        k_q8_read<__half, FMT><<<grid, kReadThreads, 0, s>>>(codes, scale, heads, max_seq, hd_log2, block_log2, start, n, (__half *)out);
-    else
-        k_q8_read<__nv_bfloat16, FMT><<<grid, kReadThreads, 0, s>>>(codes, scale, heads, max_seq, hd_log2, block_log2, start, n,
-                                                                  (__nv_bfloat16 *)out);
+    const dim3 grid((a.n + kReadThreads * kReadUnits - 1) / (kReadThreads * kReadUnits), a.heads);
+    if (dtype == SP_DTYPE_F32) k_q8_read<float, FMT><<<grid, kReadThreads, 0, s>>>(a);
+    else if (dtype == SP_DTYPE_F16) k_q8_read<__half, FMT><<<grid, kReadThreads, 0, s>>>(a);
+    else k_q8_read<__nv_bfloat16, FMT><<<grid, kReadThreads, 0, s>>>(a);
 }
 
 }  // namespace
@@ -399,13 +552,16 @@ extern "C" int sp_cuda_q8_read_kv_tokens(const sp_cuda_q8_cache_t *qc, int which
     const long long slot = (long long)seq * l.heads;
     const uint8_t *codes = (which ? l.v : l.k) + slot * l.max_seq * hd;
     const float *scale = (which ? l.v_scale : l.k_scale) + slot * (l.max_seq >> l.block_log2);
-    const long long n = (long long)n_tok * l.heads * hd / 4;
-    const long long ctas = (n + kReadThreads - 1) / kReadThreads;
-    const unsigned grid = (unsigned)(ctas < 0x7fffffff ? ctas : 0x7fffffff);
+    const int el = dtype == SP_DTYPE_F32 ? 4 : 2;
+    const int per = hd * el / 16;                    // units of a position and head
     cudaStream_t s = (cudaStream_t)qc->stream;
-    if (qc->format == SP_Q8_INT8)
-        launch_read<SP_Q8_INT8>(codes, scale, l.heads, l.max_seq, hd_log2, l.block_log2, start_pos, n, d_out, dtype, grid, s);
-    else
-        launch_read<SP_Q8_E4M3>(codes, scale, l.heads, l.max_seq, hd_log2, l.block_log2, start_pos, n, d_out, dtype, grid, s);
+    // as many positions at a time as 32-bit unit numbers reach
+    const int most = 0x7fffffff / per;
+    for (long long t = 0; t < n_tok; t += most) {
+        ReadArgs a = {codes, scale, (char *)d_out + t * per * l.heads * 16, l.heads, l.max_seq, hd_log2, l.block_log2,
+                      (int)(start_pos + t), (unsigned)((n_tok - t < most ? n_tok - t : most) * per)};
+        if (qc->format == SP_Q8_INT8) launch_read<SP_Q8_INT8>(a, dtype, s);
+        else launch_read<SP_Q8_E4M3>(a, dtype, s);
+    }
     return sp_check_cuda(cudaGetLastError(), "q8_read launch");
 }

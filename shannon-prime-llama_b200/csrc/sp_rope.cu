@@ -234,9 +234,9 @@ extern "C" int sp_cuda_rope_axes(const sp_rope_axes_t *ra, const int *d_pos, int
     a.n_tokens = n_tokens;
     a.inverse = inverse;
     const int n_pairs = ra->rot_dim / 2;
-    // One sincospif for each thread where there are tokens for several CTAs
-    // on every SM; a CTA for each token below that.
-    a.tokens_per_cta = 1;
+    // As many tokens for a CTA as give each thread one sincospif, where there
+    // are CTAs for all the SMs' threads even so; below that a CTA for each token.
+    a.tokens_per_cta = kRopeThreads / n_pairs > 1 && n_tokens >= 2048 ? kRopeThreads / n_pairs : 1;
     const unsigned grid = (unsigned)((n_tokens + a.tokens_per_cta - 1) / a.tokens_per_cta);
     const size_t smem = sizeof(float2) * n_pairs * a.tokens_per_cta;
     cudaStream_t s = (cudaStream_t)stream;
