@@ -101,7 +101,7 @@ typedef struct {
     int           block_tokens;  /* 16, 32, 64 or 128 */
     int           n_seqs;        /* sequences held */
     int           max_seq_len;   /* positions of a sequence, rounded up to a multiple of 128 */
-    void         *d_k_cache;     /* [n_layers][n_seqs][n_heads_kv][max_seq_len][head_dim] codes */
+    void         *d_k_cache;     /* start of the one allocation: [n_layers][n_seqs][n_heads_kv][max_seq_len][head_dim] codes */
     void         *d_v_cache;
     float        *d_k_scale;     /* [n_layers][n_seqs][n_heads_kv][max_seq_len / block_tokens] */
     float        *d_v_scale;

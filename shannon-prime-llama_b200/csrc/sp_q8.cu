@@ -63,21 +63,22 @@ extern "C" int sp_cuda_q8_cache_init(sp_cuda_q8_cache_t *qc, const sp_config_t *
         (rc = sp_check_cuda(cudaDeviceGetAttribute(&qc->sm_count, cudaDevAttrMultiProcessorCount, qc->device),
                             "q8_cache_init device")))
         return rc;
-    const size_t codes = (size_t)slots * qc->max_seq_len * cfg->head_dim;
-    const size_t scales = (size_t)slots * (qc->max_seq_len / block_tokens) * sizeof(float);
-    qc->attn_ws_bytes = q8::attn_workspace_bytes(qc->sm_count, cfg->head_dim);
-    if ((rc = sp_check_cuda(cudaMalloc(&qc->d_k_cache, codes), "cudaMalloc q8 K")) ||
-        (rc = sp_check_cuda(cudaMalloc(&qc->d_v_cache, codes), "cudaMalloc q8 V")) ||
-        (rc = sp_check_cuda(cudaMalloc(&qc->d_k_scale, scales), "cudaMalloc q8 K scales")) ||
-        (rc = sp_check_cuda(cudaMalloc(&qc->d_v_scale, scales), "cudaMalloc q8 V scales")) ||
-        (rc = sp_check_cuda(cudaMalloc(&qc->d_attn_ws, qc->attn_ws_bytes), "cudaMalloc q8 workspace")) ||
-        (rc = sp_check_cuda(cudaMalloc(&qc->d_status, 16), "cudaMalloc q8 status")) ||
-        (rc = sp_check_cuda(cudaMemset(qc->d_k_cache, 0, codes), "q8_cache_init")) ||
-        (rc = sp_check_cuda(cudaMemset(qc->d_v_cache, 0, codes), "q8_cache_init")) ||
-        (rc = sp_check_cuda(cudaMemset(qc->d_k_scale, 0, scales), "q8_cache_init")) ||
-        (rc = sp_check_cuda(cudaMemset(qc->d_v_scale, 0, scales), "q8_cache_init")) ||
-        (rc = sp_check_cuda(cudaMemset(qc->d_attn_ws, 0, qc->attn_ws_bytes), "q8_cache_init")) ||
-        (rc = sp_check_cuda(cudaMemset(qc->d_status, 0, 16), "q8_cache_init")) ||
+    // One allocation, in the order of the fields; every part on a 256-byte boundary.
+    auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
+    const size_t codes = up((size_t)slots * qc->max_seq_len * cfg->head_dim);
+    const size_t scales = up((size_t)slots * (qc->max_seq_len / block_tokens) * sizeof(float));
+    qc->attn_ws_bytes = up(q8::attn_workspace_bytes(qc->sm_count, cfg->head_dim));
+    char *base = nullptr;
+    if ((rc = sp_check_cuda(cudaMalloc(&base, 2 * codes + 2 * scales + 256 + qc->attn_ws_bytes), "cudaMalloc q8 cache")))
+        return rc;
+    qc->d_k_cache = base;
+    qc->d_v_cache = base + codes;
+    qc->d_k_scale = (float *)(base + 2 * codes);
+    qc->d_v_scale = (float *)(base + 2 * codes + scales);
+    qc->d_status = (unsigned int *)(base + 2 * codes + 2 * scales);
+    qc->d_attn_ws = base + 2 * codes + 2 * scales + 256;
+    // of the workspace only the counters at its start have to be zero
+    if ((rc = sp_check_cuda(cudaMemset(base, 0, 2 * codes + 2 * scales + 256 + q8::kCounterBytes), "q8_cache_init")) ||
         (rc = sp_check_cuda(cudaDeviceSynchronize(), "q8_cache_init"))) {
         sp_cuda_q8_cache_free(qc);
         return rc;
@@ -89,11 +90,6 @@ extern "C" void sp_cuda_q8_cache_free(sp_cuda_q8_cache_t *qc)
 {
     if (!qc) return;
     cudaFree(qc->d_k_cache);
-    cudaFree(qc->d_v_cache);
-    cudaFree(qc->d_k_scale);
-    cudaFree(qc->d_v_scale);
-    cudaFree(qc->d_attn_ws);
-    cudaFree(qc->d_status);
     qc->d_k_cache = qc->d_v_cache = nullptr;
     qc->d_k_scale = qc->d_v_scale = nullptr;
     qc->d_attn_ws = nullptr;

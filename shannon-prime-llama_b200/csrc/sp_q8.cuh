@@ -8,6 +8,9 @@
 
 namespace q8 {
 
+constexpr int kMaxCtas = 1024;               // most CTAs of an attention grid
+constexpr size_t kCounterBytes = kMaxCtas * sizeof(unsigned);   // at the start of its workspace
+
 constexpr float kScaleMin = 0x1p-40f, kScaleMax = 0x1p40f;
 
 __host__ __device__ constexpr float code_max(int format) { return format == SP_Q8_INT8 ? 127.0f : 448.0f; }

@@ -576,7 +576,7 @@ size_t attn_workspace_bytes(int sm_count, int head_dim)
 {
     const size_t few = (size_t)2 * 3 * sm_count * 32 * (head_dim + 2) * sizeof(float);
     const size_t many = (size_t)2 * sm_count * 256 * (head_dim + 2) * sizeof(float);
-    return kMaxCtas * sizeof(unsigned) + split_bytes(sm_count) + (few > many ? few : many);
+    return kCounterBytes + split_bytes(sm_count) + (few > many ? few : many);
 }
 }  // namespace q8
 
@@ -605,7 +605,7 @@ extern "C" int sp_cuda_q8_attn(const sp_cuda_q8_cache_t *qc, int layer, const sp
     const int G = n_q_heads / H;
     AttnArgs a = {q8::layer_of(qc, layer), q8::batch_of(qc, batch), d_q, d_out, d_lse, q_stride, out_stride,
                   n_q_heads, G, logit_scale, causal, window, 0, (unsigned int *)qc->d_attn_ws,
-                  (float *)((char *)qc->d_attn_ws + kMaxCtas * sizeof(unsigned) + q8::split_bytes(qc->sm_count))};
+                  (float *)((char *)qc->d_attn_ws + kCounterBytes + q8::split_bytes(qc->sm_count))};
     const long long tiles = (long long)batch->n_seqs * H * (batch->max_kv / kTile + 2);
     const long long rows = (long long)batch->max_new * G;
     if (tiles > 0x7fffffff) return sp_set_error(SP_ERR_ARG, "q8_attn: %lld tiles in one call", tiles);

@@ -22,7 +22,6 @@ struct AttnArgs {
     float *partials;
 };
 
-constexpr int kMaxCtas = 1024;       // most CTAs of an attention grid
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kNone = -3.402823466e38f;    // running maximum of a row that has seen nothing
 

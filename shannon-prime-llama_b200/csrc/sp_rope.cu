@@ -78,8 +78,13 @@ struct RopeHalf {
     int heads;
 };
 
+// The plan with room for PAIRS pairs: a launch copies its arguments, and 64
+// pairs (head_dim 128) are a quarter of what the largest head has.
+template <int PAIRS>
 struct RopeArgs {
-    sp_rope_axes_t ra;
+    int hd, rot;
+    uint64_t phase[PAIRS];
+    uint8_t axis[PAIRS];
     const int *pos;
     RopeHalf h[2];
     int n_tokens;
@@ -122,17 +127,17 @@ __device__ __forceinline__ void store8(T *p, const float (&x)[8])
 // and sines (one sincospif for each pair and token, not for each head), then
 // every thread rotates units of 8 adjacent elements, or 8 elements and their
 // partners half a rotation away, of any token and head.
-template <typename T, int PAIRING>
-__global__ void __launch_bounds__(kRopeThreads) k_rope_axes(const __grid_constant__ RopeArgs a)
+template <typename T, int PAIRING, int PAIRS>
+__global__ void __launch_bounds__(kRopeThreads) k_rope_axes(const __grid_constant__ RopeArgs<PAIRS> a)
 {
     extern __shared__ __align__(16) float2 cs[];       // [tokens][pairs]
-    const int n_pairs = a.ra.rot_dim / 2, hd = a.ra.head_dim, rot = a.ra.rot_dim;
+    const int n_pairs = a.rot / 2, hd = a.hd, rot = a.rot;
     const int t0 = blockIdx.x * a.tokens_per_cta;
     const int n_t = min(a.tokens_per_cta, a.n_tokens - t0);
     for (int i = threadIdx.x; i < n_t * n_pairs; i += kRopeThreads) {
         const int t = i / n_pairs, p = i - t * n_pairs;
-        const long long pos = a.pos[(long long)a.ra.axis[p] * a.n_tokens + t0 + t];
-        const uint64_t turn = (uint64_t)pos * a.ra.phase[p];
+        const long long pos = a.pos[(long long)a.axis[p] * a.n_tokens + t0 + t];
+        const uint64_t turn = (uint64_t)pos * a.phase[p];
         float s, c;
         sincospif((float)(int)(turn >> 32) * 0x1p-31f, &s, &c);
         cs[i] = make_float2(c, a.inverse ? -s : s);
@@ -190,11 +195,23 @@ __global__ void __launch_bounds__(kRopeThreads) k_rope_axes(const __grid_constan
     }
 }
 
-template <typename T>
-void launch(const RopeArgs &a, unsigned grid, size_t smem, cudaStream_t s)
+template <typename T, int PAIRS>
+void launch_pairs(const sp_rope_axes_t *ra, RopeArgs<PAIRS> &a, unsigned grid, size_t smem, cudaStream_t s)
 {
-    if (a.ra.pairing == SP_ROPE_ADJACENT) k_rope_axes<T, SP_ROPE_ADJACENT><<<grid, kRopeThreads, smem, s>>>(a);
-    else k_rope_axes<T, SP_ROPE_HALVES><<<grid, kRopeThreads, smem, s>>>(a);
+    a.hd = ra->head_dim;
+    a.rot = ra->rot_dim;
+    memcpy(a.phase, ra->phase, sizeof(a.phase));
+    memcpy(a.axis, ra->axis, sizeof(a.axis));
+    if (ra->pairing == SP_ROPE_ADJACENT) k_rope_axes<T, SP_ROPE_ADJACENT, PAIRS><<<grid, kRopeThreads, smem, s>>>(a);
+    else k_rope_axes<T, SP_ROPE_HALVES, PAIRS><<<grid, kRopeThreads, smem, s>>>(a);
+}
+
+template <int PAIRS>
+void launch(const sp_rope_axes_t *ra, RopeArgs<PAIRS> &a, int dtype, unsigned grid, size_t smem, cudaStream_t s)
+{
+    if (dtype == SP_DTYPE_F32) launch_pairs<float>(ra, a, grid, smem, s);
+    else if (dtype == SP_DTYPE_F16) launch_pairs<__half>(ra, a, grid, smem, s);
+    else launch_pairs<__nv_bfloat16>(ra, a, grid, smem, s);
 }
 
 }  // namespace
@@ -210,13 +227,10 @@ extern "C" int sp_cuda_rope_axes(const sp_rope_axes_t *ra, const int *d_pos, int
         return sp_set_error(SP_ERR_ARG, "rope_axes: dtype %d", dtype);
     if (n_tokens < 0) return sp_set_error(SP_ERR_ARG, "rope_axes: %d tokens", n_tokens);
     if (!d_q != !d_q_out || !d_k != !d_k_out) return sp_set_error(SP_ERR_ARG, "rope_axes: an input without its output");
-    RopeArgs a;
-    a.ra = *ra;
-    a.pos = d_pos;
-    a.h[0] = {d_q, d_q_out, q_stride, q_out_stride, d_q ? n_q_heads : 0};
-    a.h[1] = {d_k, d_k_out, k_stride, k_out_stride, d_k ? n_k_heads : 0};
+    RopeHalf halves[2] = {{d_q, d_q_out, q_stride, q_out_stride, d_q ? n_q_heads : 0},
+                          {d_k, d_k_out, k_stride, k_out_stride, d_k ? n_k_heads : 0}};
     const long long el = dtype == SP_DTYPE_F32 ? 4 : 2;
-    for (RopeHalf &h : a.h) {
+    for (RopeHalf &h : halves) {
         if (!h.in) continue;
         const long long row = (long long)h.heads * ra->head_dim;
         if (h.heads < 1 || h.heads > 65536) return sp_set_error(SP_ERR_ARG, "rope_axes: %d heads", h.heads);
@@ -231,17 +245,28 @@ extern "C" int sp_cuda_rope_axes(const sp_rope_axes_t *ra, const int *d_pos, int
     }
     if (n_tokens == 0 || (!d_q && !d_k)) return SP_OK;
     if (!d_pos) return sp_set_error(SP_ERR_ARG, "rope_axes: no positions");
-    a.n_tokens = n_tokens;
-    a.inverse = inverse;
     const int n_pairs = ra->rot_dim / 2;
     // As many tokens for a CTA as give each thread one sincospif, where there
     // are CTAs for all the SMs' threads even so; below that a CTA for each token.
-    a.tokens_per_cta = kRopeThreads / n_pairs > 1 && n_tokens >= 2048 ? kRopeThreads / n_pairs : 1;
-    const unsigned grid = (unsigned)((n_tokens + a.tokens_per_cta - 1) / a.tokens_per_cta);
-    const size_t smem = sizeof(float2) * n_pairs * a.tokens_per_cta;
+    const int each = kRopeThreads / n_pairs > 1 && n_tokens >= 2048 ? kRopeThreads / n_pairs : 1;
+    const unsigned grid = (unsigned)((n_tokens + each - 1) / each);
+    const size_t smem = sizeof(float2) * n_pairs * each;
     cudaStream_t s = (cudaStream_t)stream;
-    if (dtype == SP_DTYPE_F32) launch<float>(a, grid, smem, s);
-    else if (dtype == SP_DTYPE_F16) launch<__half>(a, grid, smem, s);
-    else launch<__nv_bfloat16>(a, grid, smem, s);
+    auto go = [&](auto &a) {
+        a.pos = d_pos;
+        a.h[0] = halves[0];
+        a.h[1] = halves[1];
+        a.n_tokens = n_tokens;
+        a.tokens_per_cta = each;
+        a.inverse = inverse;
+        launch(ra, a, dtype, grid, smem, s);
+    };
+    if (n_pairs <= 64) {
+        RopeArgs<64> a;
+        go(a);
+    } else {
+        RopeArgs<SP_MAX_HEAD_DIM / 2> a;
+        go(a);
+    }
     return sp_check_cuda(cudaGetLastError(), "rope_axes launch");
 }

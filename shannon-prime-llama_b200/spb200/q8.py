@@ -26,13 +26,17 @@ def _dtype(t) -> int:
 
 
 def _rows(t, heads, head_dim: int, what: str) -> int:
-    """The token stride of t [n_tokens][heads][head_dim], whose rows lie together."""
-    if t.dim() != 3 or t.shape[2] != head_dim or (heads is not None and t.shape[1] != heads):
-        raise ValueError(f"{what}: shape {tuple(t.shape)}, not [tokens][{heads or 'heads'}][{head_dim}]")
-    s = t.stride()
-    if not t.is_cuda or (t.numel() and (s[2] != 1 or (t.shape[1] > 1 and s[1] != head_dim))):
-        raise ValueError(f"{what}: a token's heads must lie together in device memory")
-    return s[0] if t.shape[0] > 1 else 0
+    """The token stride of t [n_tokens][heads][head_dim] (0: dense), whose rows lie together."""
+    sh = t.shape
+    if len(sh) != 3 or sh[2] != head_dim or (heads is not None and sh[1] != heads):
+        raise ValueError(f"{what}: shape {tuple(sh)}, not [tokens][{heads or 'heads'}][{head_dim}]")
+    if t.is_cuda:
+        if t.is_contiguous():
+            return 0
+        s = t.stride()
+        if s[2] == 1 and (sh[1] == 1 or s[1] == head_dim):
+            return s[0]
+    raise ValueError(f"{what}: a token's heads must lie together in device memory")
 
 
 class RopeAxes:
@@ -55,29 +59,28 @@ class RopeAxes:
         None) at positions pos (int32 [axes][tokens]).  The outputs are new
         tensors unless given; an output may be its input.  Returns both."""
         import torch
-        t = q if q is not None else k
+        t = k if q is None else q
         n = 0 if t is None else t.shape[0]
-        if pos.dtype != torch.int32 or tuple(pos.shape) != (self.n_axes, n) or not pos.is_contiguous() or not pos.is_cuda:
+        if pos.dtype is not torch.int32 or pos.shape != (self.n_axes, n) or not (pos.is_cuda and pos.is_contiguous()):
             raise ValueError(f"pos must be a contiguous int32 CUDA tensor [{self.n_axes}][{n}]")
-        a, dt = [], 0
-        for name, x, y in (("q", q, q_out), ("k", k, k_out)):
-            if x is None:
-                a.append((0, 0, 0, 0, 0))
-                continue
-            if y is None:
-                y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-            if name == "q":
-                q_out = y
-            else:
-                k_out = y
-            if x.shape[0] != n or y.shape != x.shape or y.dtype != x.dtype or x.dtype != t.dtype:
-                raise ValueError(f"{name}: inputs and outputs must have one type and {n} tokens")
-            dt = _dtype(x)
-            a.append((x.data_ptr(), _rows(x, None, self.head_dim, name), x.shape[1], y.data_ptr(),
-                      _rows(y, None, self.head_dim, name)))
-        (qp, qs, hq, qo, qos), (kp, ks, hk, ko, kos) = a
-        rc = self._call(self._ref, pos.data_ptr(), n, qp, qs, hq, qo, qos, kp, ks, hk, ko, kos, dt, int(inverse),
-                        _stream_ptr(stream))
+        hd = self.head_dim
+        qp = qs = hq = qo = qos = kp = ks = hk = ko = kos = 0
+        if q is not None:
+            if q_out is None:
+                q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            qs, qos, hq = _rows(q, None, hd, "q"), _rows(q_out, q.shape[1], hd, "q_out"), q.shape[1]
+            qp, qo = q.data_ptr(), q_out.data_ptr()
+            if q_out.dtype is not q.dtype or q_out.shape[0] != n:
+                raise ValueError("q and its output must have one type and number of tokens")
+        if k is not None:
+            if k_out is None:
+                k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+            ks, kos, hk = _rows(k, None, hd, "k"), _rows(k_out, k.shape[1], hd, "k_out"), k.shape[1]
+            kp, ko = k.data_ptr(), k_out.data_ptr()
+            if k_out.dtype is not k.dtype or k_out.shape[0] != n or k.shape[0] != n or k.dtype is not t.dtype:
+                raise ValueError("q, k and their outputs must have one type and number of tokens")
+        rc = self._call(self._ref, pos.data_ptr(), n, qp, qs, hq, qo, qos, kp, ks, hk, ko, kos,
+                        0 if t is None else _dtype(t), 1 if inverse else 0, 0 if stream is None else stream.cuda_stream)
         if rc:
             check(rc, "sp_cuda_rope_axes")
         return q_out, k_out
@@ -147,12 +150,12 @@ class Q8Cache:
     def write_kv_tokens(self, layer: int, batch: Q8Batch, k, v) -> None:
         """k, v: [n_tokens][n_heads_kv][head_dim] (f32/f16/bf16, one token stride;
         either may be None)."""
-        t = k if k is not None else v
+        t = v if k is None else k
         if t is None:
             return
         stride = _rows(t, self.n_heads_kv, self.head_dim, "k")
-        if k is not None and v is not None and (v.dtype != k.dtype or _rows(v, self.n_heads_kv, self.head_dim, "v") != stride
-                                                or v.shape[0] != k.shape[0]):
+        if k is not None and v is not None and (v.dtype is not k.dtype or v.shape[0] != k.shape[0]
+                                                or _rows(v, self.n_heads_kv, self.head_dim, "v") != stride):
             raise ValueError("k and v must have one type, token stride and number of tokens")
         if t.shape[0] != batch.n_tokens:
             raise ValueError(f"{t.shape[0]} tokens, the batch has {batch.n_tokens}")
@@ -163,7 +166,7 @@ class Q8Cache:
 
     def read_kv_tokens(self, which: int, layer: int, seq: int, start_pos: int, out) -> None:
         """out: [n_tok][n_heads_kv][head_dim], contiguous (f32/f16/bf16)."""
-        if not out.is_contiguous() or tuple(out.shape[1:]) != (self.n_heads_kv, self.head_dim):
+        if _rows(out, self.n_heads_kv, self.head_dim, "out") != 0:
             raise ValueError(f"out must be contiguous [tokens][{self.n_heads_kv}][{self.head_dim}]")
         rc = self._read(self._ref, which, layer, seq, start_pos, out.shape[0], out.data_ptr(), _dtype(out))
         if rc:
@@ -173,17 +176,21 @@ class Q8Cache:
              window: int = 0, stream=None):
         """q: [n_tokens][n_q_heads][head_dim] fp16 or bf16; out the same (new unless
         given); lse: fp32 [n_tokens][n_q_heads] or None.  Returns out."""
-        import torch
+        n, hq, hd = *q.shape[:2], self.head_dim
         if out is None:
+            import torch
             out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        qs, os = _rows(q, None, self.head_dim, "q"), _rows(out, q.shape[1], self.head_dim, "out")
-        n, hq = q.shape[0], q.shape[1]
-        if n != batch.n_tokens or out.shape[0] != n or out.dtype != q.dtype:
+        qs, os = _rows(q, None, hd, "q"), _rows(out, hq, hd, "out")
+        if n != batch.n_tokens or out.shape[0] != n or out.dtype is not q.dtype:
             raise ValueError(f"q and out must have one type and the batch's {batch.n_tokens} tokens")
-        if lse is not None and (lse.dtype != torch.float32 or tuple(lse.shape) != (n, hq) or not lse.is_contiguous()):
-            raise ValueError(f"lse must be a contiguous float32 tensor [{n}][{hq}]")
-        rc = self._attn(self._ref, layer, batch.ref, q.data_ptr(), qs, hq, _dtype(q), logit_scale, int(causal), window,
-                        out.data_ptr(), os, 0 if lse is None else lse.data_ptr(), _stream_ptr(stream))
+        lp = 0
+        if lse is not None:
+            if lse.shape != (n, hq) or lse.element_size() != 4 or not (lse.is_floating_point() and lse.is_cuda
+                                                                       and lse.is_contiguous()):
+                raise ValueError(f"lse must be a contiguous float32 CUDA tensor [{n}][{hq}]")
+            lp = lse.data_ptr()
+        rc = self._attn(self._ref, layer, batch.ref, q.data_ptr(), qs, hq, _dtype(q), logit_scale, 1 if causal else 0, window,
+                        out.data_ptr(), os, lp, 0 if stream is None else stream.cuda_stream)
         if rc:
             check(rc, "sp_cuda_q8_attn")
         return out
