@@ -222,6 +222,7 @@ __global__ void __launch_bounds__(THREADS) k_q8_write(const __grid_constant__ Wr
     constexpr int kPerToken = HD / 8;
     constexpr bool kAhead = sizeof(T) == 2 || THREADS < 1024;   // 1024 threads have 64 registers
     const int unit = blockIdx.x;
+    q8::begin();
 
     // which sequence and block: a running sum of the blocks that each entry touches
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
@@ -364,31 +365,32 @@ __global__ void __launch_bounds__(THREADS) k_q8_write(const __grid_constant__ Wr
 }
 
 template <typename T, int FMT, int HD>
-void launch_write_hd(const WriteArgs &a, dim3 grid, int threads, cudaStream_t s)
+int launch_write_hd(const WriteArgs &a, dim3 grid, int threads, cudaStream_t s)
 {
-    if (threads <= 256) k_q8_write<T, FMT, HD, 256><<<grid, threads, 0, s>>>(a);
+    if (threads <= 256) return q8::launch("q8_write launch", k_q8_write<T, FMT, HD, 256>, grid, threads, 0, s, a);
     if constexpr (HD >= 128) {
-        if (threads == 512) k_q8_write<T, FMT, HD, 512><<<grid, threads, 0, s>>>(a);
+        if (threads == 512) return q8::launch("q8_write launch", k_q8_write<T, FMT, HD, 512>, grid, threads, 0, s, a);
     }
     if constexpr (HD == 256) {
-        if (threads == 1024) k_q8_write<T, FMT, HD, 1024><<<grid, threads, 0, s>>>(a);
+        if (threads == 1024) return q8::launch("q8_write launch", k_q8_write<T, FMT, HD, 1024>, grid, threads, 0, s, a);
     }
+    return SP_ERR_UNSUPPORTED;
 }
 
 template <typename T, int FMT>
-void launch_write(const WriteArgs &a, int hd, dim3 grid, int threads, cudaStream_t s)
+int launch_write(const WriteArgs &a, int hd, dim3 grid, int threads, cudaStream_t s)
 {
-    if (hd == 64) launch_write_hd<T, FMT, 64>(a, grid, threads, s);
-    else if (hd == 128) launch_write_hd<T, FMT, 128>(a, grid, threads, s);
-    else launch_write_hd<T, FMT, 256>(a, grid, threads, s);
+    if (hd == 64) return launch_write_hd<T, FMT, 64>(a, grid, threads, s);
+    if (hd == 128) return launch_write_hd<T, FMT, 128>(a, grid, threads, s);
+    return launch_write_hd<T, FMT, 256>(a, grid, threads, s);
 }
 
 template <int FMT>
-void launch_write_of(const WriteArgs &a, int dtype, int hd, dim3 grid, int threads, cudaStream_t s)
+int launch_write_of(const WriteArgs &a, int dtype, int hd, dim3 grid, int threads, cudaStream_t s)
 {
-    if (dtype == SP_DTYPE_F32) launch_write<float, FMT>(a, hd, grid, threads, s);
-    else if (dtype == SP_DTYPE_F16) launch_write<__half, FMT>(a, hd, grid, threads, s);
-    else launch_write<__nv_bfloat16, FMT>(a, hd, grid, threads, s);
+    if (dtype == SP_DTYPE_F32) return launch_write<float, FMT>(a, hd, grid, threads, s);
+    if (dtype == SP_DTYPE_F16) return launch_write<__half, FMT>(a, hd, grid, threads, s);
+    return launch_write<__nv_bfloat16, FMT>(a, hd, grid, threads, s);
 }
 
 }  // namespace
@@ -435,9 +437,8 @@ extern "C" int sp_cuda_q8_write_kv_tokens(sp_cuda_q8_cache_t *qc, int layer, con
     const dim3 grid((unsigned)units, (a.slots + a.slots_each - 1) / a.slots_each);
     const int threads = (int)(B * hd / 32);
     cudaStream_t s = (cudaStream_t)qc->stream;
-    if (qc->format == SP_Q8_INT8) launch_write_of<SP_Q8_INT8>(a, dtype, hd, grid, threads, s);
-    else launch_write_of<SP_Q8_E4M3>(a, dtype, hd, grid, threads, s);
-    return sp_check_cuda(cudaGetLastError(), "q8_write launch");
+    return qc->format == SP_Q8_INT8 ? launch_write_of<SP_Q8_INT8>(a, dtype, hd, grid, threads, s)
+                                    : launch_write_of<SP_Q8_E4M3>(a, dtype, hd, grid, threads, s);
 }
 
 // ---------------------------------------------------------------- read --
@@ -484,6 +485,7 @@ template <typename T, int FMT>
 __global__ void __launch_bounds__(kReadThreads) k_q8_read(const __grid_constant__ ReadArgs a)
 {
     constexpr int E = 16 / sizeof(T);              // codes of a unit
+    q8::begin();
     const int unit_log2 = a.hd_log2 - (E == 8 ? 3 : 2);
     const int head = blockIdx.y;
     const uint8_t *codes = a.codes + (((long long)head * a.max_seq + a.start) << a.hd_log2);
@@ -519,12 +521,11 @@ __global__ void __launch_bounds__(kReadThreads) k_q8_read(const __grid_constant_
 }
 
 template <int FMT>
-void launch_read(const ReadArgs &a, int dtype, cudaStream_t s)
+int launch_read(const ReadArgs &a, int dtype, cudaStream_t s)
 {
     const dim3 grid((a.n + kReadThreads * kReadUnits - 1) / (kReadThreads * kReadUnits), a.heads);
-    if (dtype == SP_DTYPE_F32) k_q8_read<float, FMT><<<grid, kReadThreads, 0, s>>>(a);
-    else if (dtype == SP_DTYPE_F16) k_q8_read<__half, FMT><<<grid, kReadThreads, 0, s>>>(a);
-    else k_q8_read<__nv_bfloat16, FMT><<<grid, kReadThreads, 0, s>>>(a);
+    return q8::launch("q8_read launch", dtype == SP_DTYPE_F32 ? k_q8_read<float, FMT> : dtype == SP_DTYPE_F16 ? k_q8_read<__half, FMT> : k_q8_read<__nv_bfloat16, FMT>,
+                      grid, kReadThreads, 0, s, a);
 }
 
 }  // namespace
@@ -556,8 +557,8 @@ extern "C" int sp_cuda_q8_read_kv_tokens(const sp_cuda_q8_cache_t *qc, int which
     for (long long t = 0; t < n_tok; t += most) {
         ReadArgs a = {codes, scale, (char *)d_out + t * per * l.heads * 16, l.heads, l.max_seq, hd_log2, l.block_log2,
                       (int)(start_pos + t), (unsigned)((n_tok - t < most ? n_tok - t : most) * per)};
-        if (qc->format == SP_Q8_INT8) launch_read<SP_Q8_INT8>(a, dtype, s);
-        else launch_read<SP_Q8_E4M3>(a, dtype, s);
+        rc = qc->format == SP_Q8_INT8 ? launch_read<SP_Q8_INT8>(a, dtype, s) : launch_read<SP_Q8_E4M3>(a, dtype, s);
+        if (rc) return rc;
     }
-    return sp_check_cuda(cudaGetLastError(), "q8_read launch");
+    return SP_OK;
 }

@@ -15,6 +15,33 @@ constexpr float kScaleMin = 0x1p-40f, kScaleMax = 0x1p40f;
 
 __host__ __device__ constexpr float code_max(int format) { return format == SP_Q8_INT8 ? 127.0f : 448.0f; }
 
+// Every kernel of this tier is launched as a programmatic dependent: the next
+// one's CTAs are placed while the last one's finish (about 2 us of a step's short
+// kernels).  begin() stands before any access to memory: it waits until all
+// earlier work of the stream is over and seen, and only then lets the next
+// kernel be placed, so nothing that starts early finds unfinished work behind it.
+__device__ __forceinline__ void begin()
+{
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+template <typename... P, typename... A>
+int launch(const char *what, void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t s, const A &...a)
+{
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return sp_check_cuda(cudaLaunchKernelEx(&cfg, kernel, a...), what);
+}
+
 // One layer of a cache.
 struct Layer {
     const uint8_t *k, *v;          // [n_seqs][heads][max_seq][hd]

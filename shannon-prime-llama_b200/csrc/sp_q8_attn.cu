@@ -97,6 +97,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) k_q8_attn_few(const __grid_con
     FewSmem<HD, NT, STAGES> &sm = *reinterpret_cast<FewSmem<HD, NT, STAGES> *>(smem_raw);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
     const int H = a.l.heads, G = a.group;
+    begin();
 
     // ---- this CTA's run of tiles: sum over all entries, then the entry it begins in
     unsigned total = 0;
@@ -552,8 +553,7 @@ int launch_few(const AttnArgs &a, int sms, unsigned tiles, cudaStream_t s)
     unsigned grid = (unsigned)(sms * CTAS);
     if (grid > (unsigned)kMaxCtas) grid = kMaxCtas;
     if (grid > tiles) grid = tiles;
-    kernel<<<grid, kThreads, smem, s>>>(a);
-    return sp_check_cuda(cudaGetLastError(), "q8_attn launch");
+    return q8::launch("q8_attn launch", kernel, grid, kThreads, smem, s, a);
 }
 
 template <typename T, int FMT>

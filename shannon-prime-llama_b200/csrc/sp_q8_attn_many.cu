@@ -261,6 +261,7 @@ __global__ void __launch_bounds__(Shape<HD>::Threads, 1) k_q8_attn_many(const __
     ManySmem<HD> &sm = *reinterpret_cast<ManySmem<HD> *>(smem_raw);
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     constexpr int kWarps = S::Threads / 32;
+    begin();
     Split *splits = reinterpret_cast<Split *>(a.counters + kMaxCtas) + blockIdx.x;
     if (tid == 0) splits->valid = 0;
 
@@ -784,6 +785,7 @@ template <typename T, int FMT, int HD>
 __global__ void __launch_bounds__(Shape<HD>::ROWS) k_q8_attn_join(const __grid_constant__ AttnArgs a)
 {
     using S = Shape<HD>;
+    begin();
     const Split sp = reinterpret_cast<const Split *>(a.counters + kMaxCtas)[blockIdx.x];
     const int row = threadIdx.x;
     if (!sp.valid || row >= sp.rows) return;
@@ -819,7 +821,7 @@ __global__ void __launch_bounds__(Shape<HD>::ROWS) k_q8_attn_join(const __grid_c
 }
 
 template <typename T, int FMT, int HD>
-int launch(const AttnArgs &a, int sms, cudaStream_t s)
+int launch_hd(const AttnArgs &a, int sms, cudaStream_t s)
 {
     using S = Shape<HD>;
     auto kernel = k_q8_attn_many<T, FMT, HD>;
@@ -833,19 +835,17 @@ int launch(const AttnArgs &a, int sms, cudaStream_t s)
         if (rc) return rc;
         if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_release);
     }
-    kernel<<<sms, S::Threads, smem, s>>>(a);
-    int rc = sp_check_cuda(cudaGetLastError(), "q8_attn launch");
+    const int rc = q8::launch("q8_attn launch", kernel, sms, S::Threads, smem, s, a);
     if (rc) return rc;
-    k_q8_attn_join<T, FMT, HD><<<dim3(sms, HD / 16), S::ROWS, 0, s>>>(a);
-    return sp_check_cuda(cudaGetLastError(), "q8_attn join launch");
+    return q8::launch("q8_attn join launch", k_q8_attn_join<T, FMT, HD>, dim3(sms, HD / 16), S::ROWS, 0, s, a);
 }
 
 template <typename T, int FMT>
 int launch_of(const AttnArgs &a, int hd, int sms, cudaStream_t s)
 {
-    if (hd == 64) return launch<T, FMT, 64>(a, sms, s);
-    if (hd == 128) return launch<T, FMT, 128>(a, sms, s);
-    return launch<T, FMT, 256>(a, sms, s);
+    if (hd == 64) return launch_hd<T, FMT, 64>(a, sms, s);
+    if (hd == 128) return launch_hd<T, FMT, 128>(a, sms, s);
+    return launch_hd<T, FMT, 256>(a, sms, s);
 }
 
 }  // namespace

@@ -7,7 +7,7 @@
 // the position is (a 32-bit product of position and frequency is off by
 // 4e-3 radians at position 1e5).  Its top 32 bits go through sincospif.
 #include "sp_internal.cuh"
-#include "shannon_prime_q8.h"
+#include "sp_q8.cuh"
 
 #include <atomic>
 #include <math.h>
@@ -131,6 +131,7 @@ template <typename T, int PAIRING, int PAIRS>
 __global__ void __launch_bounds__(kRopeThreads) k_rope_axes(const __grid_constant__ RopeArgs<PAIRS> a)
 {
     extern __shared__ __align__(16) float2 cs[];       // [tokens][pairs]
+    q8::begin();
     const int n_pairs = a.rot / 2, hd = a.hd, rot = a.rot;
     const int t0 = blockIdx.x * a.tokens_per_cta;
     const int n_t = min(a.tokens_per_cta, a.n_tokens - t0);
@@ -196,22 +197,22 @@ __global__ void __launch_bounds__(kRopeThreads) k_rope_axes(const __grid_constan
 }
 
 template <typename T, int PAIRS>
-void launch_pairs(const sp_rope_axes_t *ra, RopeArgs<PAIRS> &a, unsigned grid, size_t smem, cudaStream_t s)
+int launch_pairs(const sp_rope_axes_t *ra, RopeArgs<PAIRS> &a, unsigned grid, size_t smem, cudaStream_t s)
 {
     a.hd = ra->head_dim;
     a.rot = ra->rot_dim;
     memcpy(a.phase, ra->phase, sizeof(a.phase));
     memcpy(a.axis, ra->axis, sizeof(a.axis));
-    if (ra->pairing == SP_ROPE_ADJACENT) k_rope_axes<T, SP_ROPE_ADJACENT, PAIRS><<<grid, kRopeThreads, smem, s>>>(a);
-    else k_rope_axes<T, SP_ROPE_HALVES, PAIRS><<<grid, kRopeThreads, smem, s>>>(a);
+    return q8::launch("rope_axes launch", ra->pairing == SP_ROPE_ADJACENT ? k_rope_axes<T, SP_ROPE_ADJACENT, PAIRS> : k_rope_axes<T, SP_ROPE_HALVES, PAIRS>,
+                      grid, kRopeThreads, smem, s, a);
 }
 
 template <int PAIRS>
-void launch(const sp_rope_axes_t *ra, RopeArgs<PAIRS> &a, int dtype, unsigned grid, size_t smem, cudaStream_t s)
+int launch(const sp_rope_axes_t *ra, RopeArgs<PAIRS> &a, int dtype, unsigned grid, size_t smem, cudaStream_t s)
 {
-    if (dtype == SP_DTYPE_F32) launch_pairs<float>(ra, a, grid, smem, s);
-    else if (dtype == SP_DTYPE_F16) launch_pairs<__half>(ra, a, grid, smem, s);
-    else launch_pairs<__nv_bfloat16>(ra, a, grid, smem, s);
+    if (dtype == SP_DTYPE_F32) return launch_pairs<float>(ra, a, grid, smem, s);
+    if (dtype == SP_DTYPE_F16) return launch_pairs<__half>(ra, a, grid, smem, s);
+    return launch_pairs<__nv_bfloat16>(ra, a, grid, smem, s);
 }
 
 }  // namespace
@@ -259,14 +260,12 @@ extern "C" int sp_cuda_rope_axes(const sp_rope_axes_t *ra, const int *d_pos, int
         a.n_tokens = n_tokens;
         a.tokens_per_cta = each;
         a.inverse = inverse;
-        launch(ra, a, dtype, grid, smem, s);
+        return launch(ra, a, dtype, grid, smem, s);
     };
     if (n_pairs <= 64) {
         RopeArgs<64> a;
-        go(a);
-    } else {
-        RopeArgs<SP_MAX_HEAD_DIM / 2> a;
-        go(a);
+        return go(a);
     }
-    return sp_check_cuda(cudaGetLastError(), "rope_axes launch");
+    RopeArgs<SP_MAX_HEAD_DIM / 2> a;
+    return go(a);
 }
