@@ -45,7 +45,7 @@ struct ManySmem {
     unsigned char q[Shape<HD>::NQ][Shape<HD>::QB];
     unsigned char k[2][Shape<HD>::StageB], v[2][Shape<HD>::StageB];
     unsigned long long q_full[2], k_full[2], k_free[2], v_full[2], v_free[2], s_full[2], p_full[2], pv_done[2], end;
-    float4 scales[Shape<HD>::SoftWarps][Shape<HD>::BN / 16];   // of a tile: K scale, log2 of V's, 1 / V's
+    float4 scales[4][Shape<HD>::BN / 16];              // of four tiles in turn: K scale, log2 of V's, 1 / V's
     unsigned scan[32];
     unsigned tiles[256];                               // of one head of each entry of a chunk, then their prefix
     int found;
@@ -86,6 +86,10 @@ __device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t (&v)[16])
 {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
                  ::"r"(at), Q8_R8(0), Q8_R8(8) : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t at, const uint32_t (&v)[8])
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(at), Q8_R8(0) : "memory");
 }
 #undef Q8_R8
 
@@ -250,7 +254,7 @@ struct Walk {
 };
 
 // Which pairs of eight take the polynomial.
-__host__ __device__ constexpr bool kPoly(int j) { return j % 8 == 7; }
+__host__ __device__ constexpr bool kPoly(int j) { return j % 4 == 3; }
 
 template <typename T, int FMT, int HD>
 __global__ void __launch_bounds__(Shape<HD>::Threads, 1) k_q8_attn_many(const __grid_constant__ AttnArgs a)
@@ -439,155 +443,160 @@ __global__ void __launch_bounds__(Shape<HD>::Threads, 1) k_q8_attn_many(const __
             if (lane == 0) arrive(spb::smem_u32(&sm.q_full[i]));
             const int hi = !real ? 0x7fffffff : a.causal ? pos : w.e.kv_len - 1;
             const int lo = real && a.window > 0 ? pos - a.window + 1 : 0;
-            const long long slot = (long long)w.e.seq * a.l.heads + w.head;
-            const float *ksp = a.l.k_scale + slot * (a.l.max_seq >> a.l.block_log2);
-            const float *vsp = a.l.v_scale + slot * (a.l.max_seq >> a.l.block_log2);
             float m = kNone, l = 0.0f;
             const int k0 = w.k0(), k1 = w.k1();
-            // a lane for each 16 positions of a tile: their scales, loaded a tile
-            // ahead (harmless ones past the end) and passed to the others through
-            // shared memory (as shuffles, three for each 16 positions, they cost a
-            // quarter of the loop)
-            float ks = 0.0f, vs = 1.0f;
-            auto load_scales = [&](int k) {
-                const int at = w.r.start + k * BN + 16 * (lane % (BN / 16));
-                const bool in = at < w.e.kv_len;
-                ks = in ? ksp[at >> a.l.block_log2] : 0.0f;
-                vs = in ? vsp[at >> a.l.block_log2] : 1.0f;
-            };
-            load_scales(k0);
             for (int k = k0; k < k1; k++, done++) {
                 const int j0 = w.r.start + k * BN;
-                const float vc = fmaxf(vs, kScaleMin);
-                if (lane < BN / 16) sm.scales[warp][lane] = make_float4(ks, lg2(vc), __frcp_rn(vc), 0.0f);
-                __syncwarp();
-                if (k + 1 < k1) load_scales(k + 1);
+                const float4 *sc = sm.scales[done & 3];
                 const bool all = __all_sync(0xffffffffu, j0 + BN - 1 <= hi && j0 >= lo);
                 const int buf = NQ == 2 ? i : (int)(done & 1);
                 const uint32_t t_s = tmem + lanes + (NQ == 2 ? 128 : 64) * buf;
                 if (!wait(sm.s_full[buf], NQ == 2 ? done : done >> 1)) goto out;
                 fence_after();
-                // A larger maximum, of positions 32 c .. 32 c + 31 too: what the products so
-                // far have summed, and this tile's weights before them, shrink.
-                auto raise = [&](int c, bool masked) {
+                // ---- 32 positions' weights by the maximum so far.  True where 16 of them
+                // sum up to more than 2^12, which no weight passes otherwise (well inside
+                // fp16): the maximum is too small.
+                auto weights = [&](const uint32_t(&u)[32], int c, uint32_t(&p)[16], float &sum) {
+                    bool over = false;
+                    sum = 0.0f;
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const float4 now = sc[2 * c + h];
+                        const float fg = now.x * mul, off = now.y - m;
+                        F2 part = {0.0f, 0.0f};
+#pragma unroll
+                        for (int j = 8 * h; j < 8 * h + 8; j++) {
+                            F2 x = fma2({__uint_as_float(u[2 * j]), __uint_as_float(u[2 * j + 1])}, {fg, fg}, {off, off});
+                            if (kPoly(j)) {
+                                x = exp2_poly(x);
+                            } else {
+                                x.x = ex2(x.x);
+                                x.y = ex2(x.y);
+                            }
+                            part = add2(part, x);
+                            const __half2 hw = __floats2half2_rn(x.x, x.y);
+                            p[j] = *reinterpret_cast<const uint32_t *>(&hw);
+                        }
+                        over |= part.x + part.y > 4096.0f;
+                        sum = fmaf(part.x + part.y, now.z, sum);
+                    }
+                    return over;
+                };
+                // ---- the same where positions are masked or the maximum has to grow: it is
+                // found first, and what the products so far have summed, and this tile's
+                // weights before these, shrink.
+                auto careful = [&](int c) {
                     float top = kNone;
 #pragma unroll 1
                     for (int h = 2 * c; h < 2 * c + 2; h++) {
-                        const float4 sc = sm.scales[warp][h];
-                        const float fg = sc.x * mul, lg = sc.y;
+                        const float fg = sc[h].x * mul, lg = sc[h].y;
                         uint32_t v[16];
                         tmem_ld16(t_s + 16 * h, v);
                         wait_ld16(v);
 #pragma unroll
                         for (int j = 0; j < 16; j++) {
                             const int at = j0 + 16 * h + j;
-                            if (!masked || (at <= hi && at >= lo)) top = fmaxf(top, fmaf(__uint_as_float(v[j]), fg, lg));
+                            if (at <= hi && at >= lo) top = fmaxf(top, fmaf(__uint_as_float(v[j]), fg, lg));
                         }
                     }
                     const bool up = top > m + 4.0f;         // a sum over 2^12 has a weight over 2^8
-                    const float fix = up ? ex2(m - top) : 1.0f;
-                    if (up) m = top;
-                    l *= fix;
-                    if (k > k0) {
-                        if (!wait_values(done - 1)) return false;
-                        fence_after();
+                    if (__any_sync(0xffffffffu, up)) {
+                        const float fix = up ? ex2(m - top) : 1.0f;
+                        if (up) m = top;
+                        l *= fix;
+                        if (k > k0) {
+                            if (!wait_values(done - 1)) return false;
+                            fence_after();
 #pragma unroll 1
-                        for (int d = 0; d < HD; d += 16) {
+                            for (int d = 0; d < HD; d += 16) {
+                                uint32_t v[16];
+                                tmem_ld16(t_o + d, v);
+                                wait_ld16(v);
+#pragma unroll
+                                for (int j = 0; j < 16; j++) v[j] = __float_as_uint(__uint_as_float(v[j]) * fix);
+                                tmem_st16(t_o + d, v);
+                            }
+                        }
+                        wait_st();
+                        const __half2 x = __float2half2_rn(fix);
+#pragma unroll 1
+                        for (int d = 0; d < 16 * c; d += 16) {
                             uint32_t v[16];
-                            tmem_ld16(t_o + d, v);
+                            tmem_ld16(t_s + d, v);
                             wait_ld16(v);
 #pragma unroll
-                            for (int j = 0; j < 16; j++) v[j] = __float_as_uint(__uint_as_float(v[j]) * fix);
-                            tmem_st16(t_o + d, v);
+                            for (int j = 0; j < 16; j++) {
+                                const __half2 y = __hmul2(*reinterpret_cast<const __half2 *>(&v[j]), x);
+                                v[j] = *reinterpret_cast<const uint32_t *>(&y);
+                            }
+                            tmem_st16(t_s + d, v);
                         }
                     }
-                    wait_st();
-                    const __half2 x = __float2half2_rn(fix);
 #pragma unroll 1
-                    for (int d = 0; d < 16 * c; d += 16) {
-                        uint32_t v[16];
-                        tmem_ld16(t_s + d, v);
+                    for (int h = 2 * c; h < 2 * c + 2; h++) {
+                        const float fg = sc[h].x * mul, off = sc[h].y - m;
+                        uint32_t v[16], p[8];
+                        tmem_ld16(t_s + 16 * h, v);
                         wait_ld16(v);
+                        float sum = 0.0f;
 #pragma unroll
-                        for (int j = 0; j < 16; j++) {
-                            const __half2 y = __hmul2(*reinterpret_cast<const __half2 *>(&v[j]), x);
-                            v[j] = *reinterpret_cast<const uint32_t *>(&y);
+                        for (int j = 0; j < 16; j += 2) {
+                            const int at = j0 + 16 * h + j;
+                            const float x = at > hi || at < lo ? 0.0f : ex2(fmaf(__uint_as_float(v[j]), fg, off));
+                            const float y = at + 1 > hi || at + 1 < lo ? 0.0f : ex2(fmaf(__uint_as_float(v[j + 1]), fg, off));
+                            sum += x + y;
+                            const __half2 hw = __floats2half2_rn(x, y);
+                            p[j / 2] = *reinterpret_cast<const uint32_t *>(&hw);
                         }
-                        tmem_st16(t_s + d, v);
+                        l = fmaf(sum, sc[h].z, l);
+                        tmem_st8(t_s + 8 * h, p);            // over scores already read
                     }
                     return true;
                 };
-                // ---- 32 positions at a time: weights by the maximum so far; where 16 of
-                // them sum up to more than 2^12 the maximum is raised and they are taken
-                // again (no weight passes 2^12 otherwise, well inside fp16)
-                auto weights = [&](auto masked) {
-                    constexpr bool kMasked = decltype(masked)::value;
-                    uint32_t u[32];
-                    tmem_ld32(t_s, u);
-                    // the scales of 32 positions, read a step ahead
-                    const float4 *sc = sm.scales[warp];
-                    float4 next[2] = {sc[0], sc[1]};
-                    // not unrolled: the instruction cache is what several roles at once
-                    // are short of
-#pragma unroll 1
+                if (all && k > k0) {
+                    uint32_t u[2][32];
+                    tmem_ld32(t_s, u[0]);
+#pragma unroll
                     for (int c = 0; c < BN / 32; c++) {
                         uint32_t p[16];
                         float sum;
-                        const float4 now[2] = {next[0], next[1]};
-                        wait_ld32(u);
+                        wait_ld32(u[c & 1]);
+                        if (c + 1 < BN / 32) tmem_ld32(t_s + 32 * (c + 1), u[(c + 1) & 1]);
+                        const bool over = weights(u[c & 1], c, p, sum);
+                        if (__any_sync(0xffffffffu, over)) {
+                            if (!careful(c)) goto out;
+                        } else {
+                            l += sum;
+                            tmem_st16(t_s + 16 * c, p);
+                        }
+                    }
+                } else {
+                    // a unit's first tile in this run, and tiles with masked positions
 #pragma unroll 1
-                        for (int again = 0;; again = 1) {
-                            F2 x[16];
-                            float fg[2], off[2];
+                    for (int c = 0; c < BN / 32; c++) {
+                        const int at = j0 + 32 * c;
+                        uint32_t p[16];
+                        if (__all_sync(0xffffffffu, !real || at > hi || at + 31 < lo)) {
 #pragma unroll
-                            for (int h = 0; h < 2; h++) {
-                                fg[h] = now[h].x * mul;
-                                off[h] = now[h].y - m;
-                            }
-#pragma unroll
-                            for (int j = 0; j < 16; j++) {
-                                x[j] = fma2({__uint_as_float(u[2 * j]), __uint_as_float(u[2 * j + 1])}, {fg[j / 8], fg[j / 8]}, {off[j / 8], off[j / 8]});
-                                if (kMasked) {
-                                    const int at = j0 + 32 * c + 2 * j;
-                                    if (at > hi || at < lo) x[j].x = -INFINITY;
-                                    if (at + 1 > hi || at + 1 < lo) x[j].y = -INFINITY;
-                                }
-                            }
-                            if (c + 1 < BN / 32) tmem_ld32(t_s + 32 * (c + 1), u);
-                            if (c + 1 < BN / 32) next[0] = sc[2 * c + 2], next[1] = sc[2 * c + 3];
-                            bool over = false;
-                            sum = 0.0f;
-#pragma unroll
-                            for (int h = 0; h < 2; h++) {
-                                F2 part = {0.0f, 0.0f};
-#pragma unroll
-                                for (int j = 8 * h; j < 8 * h + 8; j++) {
-                                    if (!kMasked && kPoly(j)) {
-                                        x[j] = exp2_poly(x[j]);
-                                    } else {
-                                        x[j].x = ex2(x[j].x);
-                                        x[j].y = ex2(x[j].y);
-                                    }
-                                    part = add2(part, x[j]);
-                                    const __half2 hw = __floats2half2_rn(x[j].x, x[j].y);
-                                    p[j] = *reinterpret_cast<const uint32_t *>(&hw);
-                                }
-                                over |= part.x + part.y > 4096.0f;
-                                sum = fmaf(part.x + part.y, now[h].z, sum);
-                            }
-                            // once: exponents past 2^26 no longer differ from the maximum by
-                            // less than their own rounding
-                            if (again || !__any_sync(0xffffffffu, over)) break;
-                            if (!raise(c, kMasked)) return false;
+                            for (int j = 0; j < 16; j++) p[j] = 0;
+                            tmem_st16(t_s + 16 * c, p);
+                            continue;
+                        }
+                        bool slow = !__all_sync(0xffffffffu, at + 31 <= hi && at >= lo && m > kNone);
+                        if (!slow) {
+                            uint32_t u[32];
+                            float sum;
                             tmem_ld32(t_s + 32 * c, u);
                             wait_ld32(u);
+                            slow = __any_sync(0xffffffffu, weights(u, c, p, sum));
+                            if (!slow) {
+                                l += sum;
+                                tmem_st16(t_s + 16 * c, p);
+                            }
                         }
-                        l += sum;
-                        tmem_st16(t_s + 16 * c, p);
+                        if (slow && !careful(c)) goto out;
                     }
-                    return true;
-                };
-                if (!(all ? weights(std::false_type{}) : weights(std::true_type{}))) goto out;
+                }
                 wait_st();
                 fence_before();
                 __syncwarp();
@@ -697,6 +706,19 @@ __global__ void __launch_bounds__(Shape<HD>::Threads, 1) k_q8_attn_many(const __
             const int k0 = w.k0(), k1 = w.k1();
             load(kx, kp + (long long)k0 * BN * HD);
             load(vx, vp + (long long)k0 * BN * HD);
+            // the first warp's lanes: the scales of 16 positions each, a tile ahead
+            // (harmless ones past the end).  Four places: those of tile n are written
+            // after tile n - 2's scores were taken, so after tile n - 3's weights.
+            const float *ksp = a.l.k_scale + slot * (a.l.max_seq >> a.l.block_log2);
+            const float *vsp = a.l.v_scale + slot * (a.l.max_seq >> a.l.block_log2);
+            float ks = 0.0f, vs = 1.0f;
+            auto load_scales = [&](int k) {
+                const int at = w.r.start + k * BN + 16 * lane;
+                const bool in = cw == 0 && lane < BN / 16 && at < w.e.kv_len;
+                ks = in ? ksp[at >> a.l.block_log2] : 0.0f;
+                vs = in ? vsp[at >> a.l.block_log2] : 1.0f;
+            };
+            load_scales(k0);
             // codes of V past the end may be NaN, which a weight of 0 does not undo
             auto no_nan = [&](int j0) {
                 if (FMT == SP_Q8_E4M3 && j0 + BN > w.e.kv_len) {
@@ -708,6 +730,10 @@ __global__ void __launch_bounds__(Shape<HD>::Threads, 1) k_q8_attn_many(const __
             for (int k = k0; k < k1; k++, done++) {
                 const int st = done & 1;
                 if (done >= 2 && !wait(sm.k_free[st], done / 2 - 1)) goto out;
+                if (cw == 0 && lane < BN / 16) {
+                    const float v = fmaxf(vs, kScaleMin);
+                    sm.scales[done & 3][lane] = make_float4(ks, lg2(v), __frcp_rn(v), 0.0f);
+                }
                 store(kx, sm.k[st], sm.k_full[st]);
                 if (done >= 2 && !wait(sm.v_free[st], done / 2 - 1)) goto out;
                 no_nan(w.r.start + k * BN);
@@ -716,6 +742,7 @@ __global__ void __launch_bounds__(Shape<HD>::Threads, 1) k_q8_attn_many(const __
                 if (k + 1 < k1) {
                     load(kx, kp + (long long)(k + 1) * BN * HD);
                     load(vx, vp + (long long)(k + 1) * BN * HD);
+                    load_scales(k + 1);
                 }
             }
         }
