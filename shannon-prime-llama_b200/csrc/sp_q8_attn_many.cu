@@ -224,6 +224,24 @@ __device__ __forceinline__ Rows rows_of(const AttnArgs &a, const Entry &e, int q
     return r;
 }
 
+// Token and query head (of the KV head's) of the unit's row rr: one division for
+// the unit, then a multiplication each (exact for rr + group < 2^32 / group).
+struct RowMap {
+    int t0, r0, group;
+    unsigned inv;
+    __device__ __forceinline__ RowMap(int row0, int g) : group(g), inv(0xffffffffu / g + 1)
+    {
+        t0 = row0 / g;
+        r0 = row0 - t0 * g;
+    }
+    __device__ __forceinline__ void at(int rr, int &token, int &head) const
+    {
+        const unsigned y = r0 + rr, q = group == 1 ? y : __umulhi(y, inv);
+        token = t0 + q;
+        head = y - q * group;
+    }
+};
+
 // Walks the units of a run: every role goes through the same ones.
 template <int HD>
 struct Walk {
@@ -394,10 +412,13 @@ __global__ void __launch_bounds__(Shape<HD>::Threads, 1) k_q8_attn_many(const __
         // phases apart: the buffers have a barrier each.
         auto wait_values = [&](unsigned n) { return NQ == 2 ? wait(sm.pv_done[i], n) : wait(sm.pv_done[n & 1], n >> 1); };
         for (; w.more(); w.next(a)) {
-            const int row = w.r.row0 + 128 * i + r;
+            const RowMap map(w.r.row0, a.group);
             const bool real = 128 * i + r < w.r.rows;
-            const int tok = w.e.q0 + row / a.group, qh = w.head * a.group + row % a.group;
-            const int first = w.e.kv_len - w.e.n, pos = first + row / a.group;
+            int tok, qh;
+            map.at(128 * i + r, tok, qh);
+            const int pos = w.e.kv_len - w.e.n + tok;
+            tok += w.e.q0;
+            qh += w.head * a.group;
             // ---- the warp's 32 rows of queries, 8 rows x 4 runs of 8 dimensions at a
             // time, into the operand's places as they are; then a thread for each
             // row scales its own to fp16
@@ -405,9 +426,10 @@ __global__ void __launch_bounds__(Shape<HD>::Threads, 1) k_q8_attn_many(const __
             unsigned char *own = sm.q[i] + (warp & 3) * 4 * S::Rows8;
 #pragma unroll 1
             for (int n = 0; n < 4; n++) {
-                const int rr = 128 * i + 32 * (warp & 3) + 8 * n + (lane >> 2), ar = w.r.row0 + rr;
-                const T *q = static_cast<const T *>(a.q) + (long long)(w.e.q0 + ar / a.group) * a.q_stride +
-                             (w.head * a.group + ar % a.group) * HD + (lane & 3) * 8;
+                const int rr = 128 * i + 32 * (warp & 3) + 8 * n + (lane >> 2);
+                int t, h;
+                map.at(rr, t, h);
+                const T *q = static_cast<const T *>(a.q) + (w.e.q0 + t) * a.q_stride + (w.head * a.group + h) * HD + (lane & 3) * 8;
                 const uint32_t dst = spb::smem_u32(own + n * S::Rows8 + (lane & 3) * S::Core + (lane >> 2) * 16), bytes = rr < w.r.rows ? 16 : 0;
 #pragma unroll
                 for (int c = 0; c < HD / 32; c++)
@@ -626,13 +648,14 @@ __global__ void __launch_bounds__(Shape<HD>::Threads, 1) k_q8_attn_many(const __
                     }
                 }
                 __syncwarp();
-                constexpr int kPieces = HD / 8;                  // of a row
+                constexpr int kPieces = HD / 8, kRowsAt = 32 / kPieces ? 32 / kPieces : 1;     // of a row; rows at a time
+                const int pc = lane % kPieces, r0 = lane / kPieces;
 #pragma unroll 4
-                for (int n = lane; n < 32 * kPieces; n += 32) {
-                    const int rr = n / kPieces, pc = n % kPieces, ar = w.r.row0 + 128 * i + 32 * (warp & 3) + rr;
-                    if (ar < w.r.row0 + w.r.rows) {
-                        T *out = static_cast<T *>(a.out) + (long long)(w.e.q0 + ar / a.group) * a.out_stride +
-                                 (w.head * a.group + ar % a.group) * HD;
+                for (int rr = r0; rr < 32; rr += kRowsAt) {
+                    int t, h;
+                    map.at(128 * i + 32 * (warp & 3) + rr, t, h);
+                    if (128 * i + 32 * (warp & 3) + rr < w.r.rows) {
+                        T *out = static_cast<T *>(a.out) + (w.e.q0 + t) * a.out_stride + (w.head * a.group + h) * HD;
                         reinterpret_cast<uint4 *>(out)[pc] = *reinterpret_cast<const uint4 *>(own + rr * HD * 2 + (pc ^ (rr & 7)) * 16);
                     }
                 }
@@ -837,7 +860,10 @@ __global__ void __launch_bounds__(Shape<HD>::ROWS) k_q8_attn_join(const __grid_c
         }
     }
     const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
-    const int rr = sp.row0 + row, tok = sp.q0 + rr / a.group, qh = sp.head * a.group + rr % a.group;
+    int tok, qh;
+    RowMap(sp.row0, a.group).at(row, tok, qh);
+    tok += sp.q0;
+    qh += sp.head * a.group;
     T x[16];
 #pragma unroll
     for (int j = 0; j < 16; j++) x[j] = T(acc[j] * inv);
