@@ -216,6 +216,14 @@ __device__ __forceinline__ uint2 encode8(float (&x)[8])
 // finds its maximum.  The next pair's input is on its way meanwhile.  (A cluster
 // of CTAs of 256 threads for the larger blocks, joining their maxima through
 // shared memory, took 1.4 times as long.)
+//
+// Memory and the chain load, maximum, barrier, codes, store bound it: 33042
+// tokens of prompts in bf16 (8 heads of 128, blocks of 32, e4m3; 195 MB) take 39
+// us, 76% of the copy rate; 8192 in 32 bits (16 heads of 256, blocks of 128,
+// int8; 336 MB) 70 us, 74%.  With places and masks found anew for each pair and
+// maxima joined by shuffles 47 and 77 us; one pair for each CTA, without the
+// next one's input on its way, 68 and 104 us.  Single tokens of 16 sequences
+// take 6.8 us, most of it the launch.
 template <typename T, int FMT, int HD, int THREADS>
 __global__ void __launch_bounds__(THREADS) k_q8_write(const __grid_constant__ WriteArgs a)
 {
@@ -262,44 +270,58 @@ __global__ void __launch_bounds__(THREADS) k_q8_write(const __grid_constant__ Wr
     const int p0 = e.kv_len - e.n, lo = blk << a.block_log2;
     const bool keeps = p0 > lo;                  // older positions stay in this block
     const int s0 = blockIdx.y * a.slots_each, s1 = min(s0 + a.slots_each, a.slots);
-    __shared__ float tops[2][THREADS / 32];
+    // maxima of the warps, which as bits are in the order of whole numbers; of two
+    // pairs in turn, so that one barrier for each pair is enough
+    __shared__ __align__(16) unsigned tops[2][THREADS / 32 < 4 ? 4 : THREADS / 32];
+    if (warps < 4 && threadIdx.x < 8 && (threadIdx.x & 3) >= warps) tops[threadIdx.x >> 2][threadIdx.x & 3] = 0;
 
-    auto load = [&](Raw8<T>(&raw)[4], int slot) {
-        const int half = slot / a.heads, head = slot - half * a.heads;
+    // this thread's groups: of the tokens row, row + step, ..., the ones to be written
+    const int row = threadIdx.x / kPerToken, step = blockDim.x / kPerToken;
+    unsigned has = 0;
 #pragma unroll
-        for (int c = 0; c < 4; c++) {
-            const int g = c * blockDim.x + threadIdx.x;
-            const int pos = lo + g / kPerToken;
-            if (pos >= p0 && pos < e.kv_len) {
-                const T *src = static_cast<const T *>(a.h[half].in) + (long long)(e.q0 + pos - p0) * a.token_stride +
-                               head * HD + (g % kPerToken) * 8;
+    for (int c = 0; c < 4; c++)
+        if (lo + row + c * step >= p0 && lo + row + c * step < e.kv_len) has |= 1u << c;
+    const long long in_at = (long long)(e.q0 + lo + row - p0) * a.token_stride + threadIdx.x % kPerToken * 8;
+    const long long in_step = (long long)step * a.token_stride;
+    int half = s0 / a.heads, head = s0 - half * a.heads, next_half = half, next_head = head;
+    auto load = [&](Raw8<T>(&raw)[4]) {
+        const T *src = static_cast<const T *>(a.h[next_half].in) + in_at + next_head * HD;
+#pragma unroll
+        for (int c = 0; c < 4; c++, src += in_step) {
+            if (has >> c & 1) {
 #pragma unroll
                 for (int i = 0; i < (int)sizeof(T) / 2; i++) raw[c].w[i] = __ldcs(reinterpret_cast<const uint4 *>(src) + i);
             }
         }
+        if (++next_head == a.heads) {
+            next_head = 0;
+            next_half++;
+        }
     };
     auto one = [&](const Raw8<T>(&raw)[4], Raw8<T>(&next)[4], int slot) {
-        const int half = slot / a.heads, head = slot - half * a.heads, odd = slot & 1;
+        const int odd = slot & 1;
         const WriteHalf &h = a.h[half];
         const long long at = (long long)e.seq * a.heads + head;
         uint8_t *codes = h.codes + (at * a.max_seq + lo) * HD;
         float *scale = h.scale + at * (a.max_seq >> a.block_log2) + blk;
+        if (++head == a.heads) {
+            head = 0;
+            half++;
+        }
         const float old = keeps ? *scale : 0.0f;
-        if (kAhead && slot + 1 < s1) load(next, slot + 1);
+        if (kAhead && slot + 1 < s1) load(next);
         Top<T> most;
 #pragma unroll
-        for (int c = 0; c < 4; c++) {
-            const int pos = lo + (c * (int)blockDim.x + (int)threadIdx.x) / kPerToken;
-            if (pos >= p0 && pos < e.kv_len) most.add(raw[c]);
-        }
-        // a thread with an infinity or NaN says so by a negative maximum of the others
+        for (int c = 0; c < 4; c++)
+            if (has >> c & 1) most.add(raw[c]);
+        // infinities and NaN do not count
         float top = most.value();
-        if (!(top <= 3.402823466e38f)) {
+        bool odd_values = !(top <= 3.402823466e38f);
+        if (odd_values) {
             top = 0.0f;
 #pragma unroll
             for (int c = 0; c < 4; c++) {
-                const int pos = lo + (c * (int)blockDim.x + (int)threadIdx.x) / kPerToken;
-                if (pos >= p0 && pos < e.kv_len) {
+                if (has >> c & 1) {
 #pragma unroll
                     for (int i = 0; i < 8; i++) {
                         const float m = fabsf(raw_at(raw[c], i));
@@ -307,20 +329,16 @@ __global__ void __launch_bounds__(THREADS) k_q8_write(const __grid_constant__ Wr
                     }
                 }
             }
-            top = -top;
         }
-        bool odd_values = __any_sync(0xffffffffu, __float_as_uint(top) >> 31);
-        top = fabsf(top);
-#pragma unroll
-        for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-        if (lane == 0) tops[odd][warp] = odd_values ? -top : top;
-        __syncthreads();
-        top = 0.0f;
-        odd_values = false;
-        for (int i = 0; i < warps; i++) {
-            odd_values |= __float_as_uint(tops[odd][i]) >> 31;
-            top = fmaxf(top, fabsf(tops[odd][i]));
+        const unsigned warp_top = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+        if (lane == 0) tops[odd][warp] = warp_top;
+        odd_values = __syncthreads_or(odd_values);
+        unsigned all_top = 0;
+        for (int i = 0; i < warps; i += 4) {
+            const uint4 w = *reinterpret_cast<const uint4 *>(&tops[odd][i]);
+            all_top = max(max(all_top, max(w.x, w.y)), max(w.z, w.w));
         }
+        top = __uint_as_float(all_top);
 
         float s = fminf(fmaxf(__fmul_rn(top, 1.0f / q8::code_max(FMT)), q8::kScaleMin), q8::kScaleMax);
         const bool grown = keeps && s > old;
@@ -331,15 +349,13 @@ __global__ void __launch_bounds__(THREADS) k_q8_write(const __grid_constant__ Wr
         if (threadIdx.x == 0) *scale = s;            // all have read the old one: the barrier above
 #pragma unroll
         for (int c = 0; c < 4; c++) {
-            const int g = c * blockDim.x + threadIdx.x;
-            const int pos = lo + g / kPerToken;
-            uint2 *dst = reinterpret_cast<uint2 *>(codes + (long long)g * 8);
+            uint2 *dst = reinterpret_cast<uint2 *>(codes) + c * blockDim.x + threadIdx.x;
             float x[8];
-            if (pos >= p0 && pos < e.kv_len) {
+            if (has >> c & 1) {
 #pragma unroll
                 for (int i = 0; i < 8; i++) x[i] = __fmul_rn(raw_at(raw[c], i), inv);
                 *dst = checked ? encode8<FMT, true>(x) : encode8<FMT, false>(x);
-            } else if (grown && pos < p0) {
+            } else if (grown && lo + row + c * step < p0) {
                 const float ratio = __fdiv_rn(old, s);
                 const uint2 w = *dst;
                 const uint8_t *b = reinterpret_cast<const uint8_t *>(&w);
@@ -351,14 +367,14 @@ __global__ void __launch_bounds__(THREADS) k_q8_write(const __grid_constant__ Wr
     };
     Raw8<T> x[4], y[4];
     if (kAhead) {
-        load(x, s0);
+        load(x);
         for (int slot = s0; slot < s1; slot += 2) {
             one(x, y, slot);
             if (slot + 1 < s1) one(y, x, slot + 1);
         }
     } else {
         for (int slot = s0; slot < s1; slot++) {
-            load(x, slot);
+            load(x);
             one(x, x, slot);
         }
     }
@@ -480,7 +496,9 @@ __device__ __forceinline__ void decode8(uint2 c, float (&x)[8])
 
 // A row of CTAs for each head.  Each thread turns kReadUnits units of codes (16
 // bytes of values each) into values; a warp's loads and stores of one unit are
-// contiguous within a position.
+// contiguous within a position.  Memory bounds it: 32768 positions of 8 heads
+// of 128, K and V, 201 MB with their values in bf16, in 36 to 41 us, 75 to 85% of
+// the copy rate (a unit for each thread, heads in turn within a position: 97 us).
 template <typename T, int FMT>
 __global__ void __launch_bounds__(kReadThreads) k_q8_read(const __grid_constant__ ReadArgs a)
 {

@@ -8,11 +8,11 @@
 //     P = 2^(S f + log2 vs - m), by the rows' own threads, back into the
 //         columns of S as fp16 (the softmax of sp_q8_attn.cu)
 //     O += P V      P from tensor memory, V from shared memory
-// Codes become fp16 once for all 256 rows: seven warps (eleven) load them, unpack them
-// in registers and store them in the core-matrix layout (8 rows of 16 bytes)
-// that serves K as the K-major and V as the MN-major operand.  One thread
-// issues the products; while a softmax warpgroup works on its 128 rows, the
-// tensor cores work on the other 128.
+// Codes become fp16 once for all 256 rows: seven warps (eleven at head_dim 256)
+// load them, unpack them in registers and store them in the core-matrix layout
+// (8 rows of 16 bytes) that serves K as the K-major and V as the MN-major
+// operand.  One thread issues the products; while a softmax warpgroup works on
+// its 128 rows, the tensor cores work on the other 128.
 #include "sp_q8_attn.cuh"
 #include "sp_bulk.cuh"
 
@@ -271,7 +271,8 @@ struct Walk {
     }
 };
 
-// Which pairs of eight take the polynomial.
+// Which pairs of weights take the polynomial: one in four, so that the special-
+// function unit and the others end together (none: 6% longer for the loop).
 __host__ __device__ constexpr bool kPoly(int j) { return j % 4 == 3; }
 
 template <typename T, int FMT, int HD>

