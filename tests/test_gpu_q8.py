@@ -589,3 +589,60 @@ def test_refusals(cuda):
     with pytest.raises(RuntimeError):
         spb200.Q8Cache(128, 1, 1, 128, block_tokens=48)
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("hd,H,G,fmt", [(256, 2, 8, "e4m3"), (128, 2, 4, "int8"), (64, 3, 2, "e4m3")])
+def test_attn_many_tiles_again_and_again(cuda, hd, H, G, fmt):
+    """Long chunks of several entries: runs that end and begin inside units, the
+    roles of the many-row kernel far apart.  Every pass gives the same bits and
+    no wait runs out."""
+    new, kv = [301, 1, 700, 95], [3000, 2500, 5000, 95]
+    cache, q, first = _run_attn(hd, H, G, 64, fmt, "f16", new, kv, scale=1.0 / np.sqrt(hd))
+    b = _batch(new, kv)
+    for _ in range(40):
+        out = cache.attn(0, b, q, logit_scale=1.0 / np.sqrt(hd))
+        assert torch.equal(out, first)
+    assert cache.status() == 0
+
+
+@pytest.mark.parametrize("most", [1, 40])
+def test_attn_many_entries(cuda, most):
+    """More entries than a CTA has threads, of many lengths, some of them empty,
+    through both kernels."""
+    new = [(0, 1, most, 1, (i * 7) % most + 1)[i % 5] for i in range(601)]
+    kv = [n + (i * 13) % 90 for i, n in enumerate(new)]
+    _run_attn(64, 1, 2, 16, "int8", "f16", new, kv, max_seq=144)
+
+
+@pytest.mark.parametrize("most", [1, 40])
+def test_write_many_entries(cuda, most):
+    n, hd, B = 601, 64, 16
+    new = [(0, 1, most, 1, (i * 7) % most + 1)[i % 5] for i in range(n)]
+    at = [(i * 13) % 90 for i in range(n)]
+    cache = spb200.Q8Cache(hd, 1, 1, 144, n_seqs=n, fmt="e4m3", block_tokens=B)
+    want = _fill(cache, 7)
+    g = torch.Generator().manual_seed(11)
+    x = [torch.randn(sum(new), 1, hd, generator=g) * s for s in (3.0, 0.4)]
+    cache.write_kv_tokens(0, _batch(new, [a + m for a, m in zip(at, new)]), x[0].cuda(), x[1].cuda())
+    assert cache.status() == 0
+    for which in (0, 1):
+        codes, scales = want[2 * which], want[2 * which + 1]
+        row = 0
+        for i, (s, m) in enumerate(zip(at, new)):
+            R.write(codes[0, i, 0], scales[0, i, 0], x[which][row:row + m, 0], s, B, "e4m3")
+            row += m
+        assert torch.equal(cache.scales(which).cpu(), scales)
+        assert torch.equal(cache.slab(which).view(torch.uint8).cpu(), codes)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+def test_example_runs(cuda, fmt):
+    """The example: rotation, write, attention over prompts and a graph of single tokens."""
+    import importlib.util
+    from pathlib import Path
+    at = Path(__file__).resolve().parent.parent / "shannon-prime-llama_b200" / "examples" / "q8_layers.py"
+    spec = importlib.util.spec_from_file_location("q8_layers", at)
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    # the output's own rounding (2^-11) and the weights' (2^-11)
+    assert mod.main(["--layers", "2", "--steps", "5", "--fmt", fmt]) <= 2.0 ** -10
