@@ -62,7 +62,8 @@ typedef struct {
 /* head_dim: a multiple of 8 up to SP_MAX_HEAD_DIM.  rot_dim: a multiple of
  * 16 up to head_dim.  sections[n_axes]: pairs of each axis, >= 0, together
  * rot_dim/2.  freq_factors: NULL or rot_dim/2 finite divisors (not zero) of the
- * frequencies.  Host only. */
+ * frequencies.  A frequency is the 32-bit float nearest to the formula's value,
+ * as in the tables that models are trained with.  Host only. */
 int sp_rope_axes_init(sp_rope_axes_t *ra, int head_dim, int rot_dim, int pairing, int n_axes,
                       const int *sections, int flags, double theta, const float *freq_factors);
 

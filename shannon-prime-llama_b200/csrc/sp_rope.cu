@@ -1,11 +1,13 @@
 // sp_rope.cu — rotary positions with several axes (shannon_prime_q8.h).
 //
 // Each pair (x, y) of a head's first rot_dim elements turns by
-// a = pos[axis] * f.  The angle is kept as a fraction of a turn in 64-bit
-// fixed point: f / 2 pi times 2^64 is rounded once on the host, and the low
-// 64 bits of position * phase are the fraction, reduced exactly however far
-// the position is (a 32-bit product of position and frequency is off by
-// 4e-3 radians at position 1e5).  Its top 32 bits go through sincospif.
+// a = pos[axis] * f, f a 32-bit float: the tables of frequencies that models
+// are trained with are such, and at position 1e5 the formula's own frequencies
+// turn by up to 3e-3 radians more or less.  The angle is kept as a fraction of a
+// turn in 64-bit fixed point: f / 2 pi times 2^64 is rounded once on the host,
+// and the low 64 bits of position * phase are the fraction, reduced exactly
+// however far the position is (a 32-bit product of position and frequency is
+// off by another 4e-3 radians there).  Its top 32 bits go through sincospif.
 #include "sp_internal.cuh"
 #include "sp_q8.cuh"
 
@@ -56,6 +58,8 @@ extern "C" int sp_rope_axes_init(sp_rope_axes_t *ra, int head_dim, int rot_dim, 
                 return sp_set_error(SP_ERR_ARG, "rope_axes_init: factor %d is %g", i, (double)freq_factors[i]);
             f /= (double)freq_factors[i];
         }
+        f = (double)(float)f;
+        if (!isfinite(f)) return sp_set_error(SP_ERR_ARG, "rope_axes_init: frequency %d is past 32-bit floats", i);
         // whole turns for each step do not matter at whole positions
         double turn = f / 6.283185307179586476925;
         turn -= floor(turn);

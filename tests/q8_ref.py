@@ -27,6 +27,7 @@ def rope(x, pos, sections, rot, pairing, interleave, ladder, theta, sign=1.0, fa
         used[a] += 1
         if factors is not None:
             f /= factors[i]
+        f = float(np.float32(f))        # frequencies are 32-bit floats
         ang = sign * pos[a].astype(np.float64)[:, None] * f
         p, r = (2 * i, 2 * i + 1) if pairing == "adjacent" else (i, i + rot // 2)
         y[..., p] = x[..., p] * np.cos(ang) - x[..., r] * np.sin(ang)

@@ -3,6 +3,7 @@ formula, the pairs' axes, and what is refused.  No GPU."""
 import ctypes as C
 from fractions import Fraction
 
+import numpy as np
 import pytest
 
 
@@ -15,7 +16,7 @@ def test_phases_match_the_ladder(built_lib):
     import math
     p = _plan(head_dim=128, sections=[64], theta=10000.0)
     for i in range(64):
-        want = Fraction(10000.0 ** (-i / 64)) / Fraction(2 * math.pi)
+        want = Fraction(float(np.float32(10000.0 ** (-i / 64)))) / Fraction(2 * math.pi)   # frequencies are 32-bit floats
         # two roundings in 64-bit floats, pow and the division (2^-52 of the value), and the
         # fixed point's last place
         assert abs(Fraction(p.phase[i], 2 ** 64) - want) <= want * Fraction(1, 2 ** 51) + Fraction(1, 2 ** 64)
@@ -34,7 +35,8 @@ def test_interleaved_axes(built_lib):
     dict(head_dim=64, sections=[12]), dict(head_dim=64, sections=[48]), dict(head_dim=64, sections=[40, -8]),
     dict(head_dim=64, sections=[8, 8, 8, 4, 4]), dict(head_dim=64, sections=[]), dict(head_dim=64, sections=[32], theta=0.0),
     dict(head_dim=64, sections=[32], theta=float("inf")), dict(head_dim=64, sections=[32], freq_factors=[0.0] * 32),
-    dict(head_dim=64, sections=[32], freq_factors=[float("nan")] * 32)])
+    dict(head_dim=64, sections=[32], freq_factors=[float("nan")] * 32),
+    dict(head_dim=64, sections=[32], freq_factors=[1e-39] * 32)])
 def test_plan_refusals(built_lib, kw):
     with pytest.raises(RuntimeError):
         _plan(**kw)
