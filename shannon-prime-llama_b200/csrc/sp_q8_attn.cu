@@ -459,12 +459,12 @@ __global__ void __launch_bounds__(kThreads, CTAS) k_q8_attn_few(const __grid_con
         const unsigned run0 = run_of_tile(runs, unit_t), run1 = run_of_tile(runs, unit_t + u.tiles - 1);
         constexpr int kSlot = 8 * NT * (HD + 2);
         auto finish = [&](int row, int d, float4 v, float top, float sum) {
-            const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;      // a sum that is NaN stays
             T w[4] = {T(v.x * inv), T(v.y * inv), T(v.z * inv), T(v.w * inv)};
             const long long tok = e.q0 + row / G;
             const int qh = head * G + row % G;
             *reinterpret_cast<uint2 *>(static_cast<T *>(a.out) + tok * a.out_stride + qh * HD + d) = *reinterpret_cast<uint2 *>(w);
-            if (a.lse && d == 0) a.lse[tok * a.n_q_heads + qh] = sum > 0.0f ? kLn2 * (top + lg2(sum)) : -INFINITY;
+            if (a.lse && d == 0) a.lse[tok * a.n_q_heads + qh] = sum == 0.0f ? -INFINITY : kLn2 * (top + lg2(sum));
         };
         // slots: a run has at most one unit that began before it and one that goes on after it
         float *part = a.partials + (2 * blockIdx.x + (unit_t >= t_begin)) * kSlot;

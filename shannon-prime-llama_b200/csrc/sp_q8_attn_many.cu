@@ -630,7 +630,7 @@ __global__ void __launch_bounds__(Shape<HD>::Threads, 1) k_q8_attn_many(const __
             fence_after();
             const bool whole = k0 == 0 && k1 == w.r.tiles;
             if (whole) {
-                const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+                const float inv = l == 0.0f ? 0.0f : 1.0f / l;      // a sum that is NaN stays
                 // through the warp's own part of the queries' place, so that a row's
                 // bytes leave together: 16-byte pieces, exchanged within groups of
                 // eight by the row to fall on different banks
@@ -661,7 +661,7 @@ __global__ void __launch_bounds__(Shape<HD>::Threads, 1) k_q8_attn_many(const __
                     }
                 }
                 __syncwarp();
-                if (real && a.lse) a.lse[(long long)tok * a.n_q_heads + qh] = l > 0.0f ? kLn2 * (m + lg2(l)) : -INFINITY;
+                if (real && a.lse) a.lse[(long long)tok * a.n_q_heads + qh] = l == 0.0f ? -INFINITY : kLn2 * (m + lg2(l));
             } else {
                 // rows side by side, so that a warp's stores are contiguous
                 float *part = a.partials + (long long)(2 * blockIdx.x + (w.unit_t >= run_begin(runs, blockIdx.x))) * S::SlotFloats;
@@ -860,7 +860,7 @@ __global__ void __launch_bounds__(Shape<HD>::ROWS) k_q8_attn_join(const __grid_c
             acc[4 * j + 3] = fmaf(x[j].w, f1, acc[4 * j + 3] * f0);
         }
     }
-    const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;      // a sum that is NaN stays
     int tok, qh;
     RowMap(sp.row0, a.group).at(row, tok, qh);
     tok += sp.q0;
@@ -871,7 +871,7 @@ __global__ void __launch_bounds__(Shape<HD>::ROWS) k_q8_attn_join(const __grid_c
     T *out = static_cast<T *>(a.out) + (long long)tok * a.out_stride + qh * HD + 16 * blockIdx.y;
     reinterpret_cast<uint4 *>(out)[0] = reinterpret_cast<const uint4 *>(x)[0];
     reinterpret_cast<uint4 *>(out)[1] = reinterpret_cast<const uint4 *>(x)[1];
-    if (a.lse && blockIdx.y == 0) a.lse[(long long)tok * a.n_q_heads + qh] = sum > 0.0f ? kLn2 * (top + lg2(sum)) : -INFINITY;
+    if (a.lse && blockIdx.y == 0) a.lse[(long long)tok * a.n_q_heads + qh] = sum == 0.0f ? -INFINITY : kLn2 * (top + lg2(sum));
 }
 
 template <typename T, int FMT, int HD>

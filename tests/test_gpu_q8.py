@@ -636,6 +636,24 @@ def test_write_many_entries(cuda, most):
 
 
 @pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("new,kv", [(1, 700), (3, 90), (100, 700)])
+def test_attn_nan_queries_stay_in_their_rows(cuda, fmt, new, kv):
+    """A query row with a NaN has NaN for its output and lse; the others are as they should be."""
+    hd, G = 128, 4
+    cache = spb200.Q8Cache(hd, 1, 1, kv, fmt=fmt, block_tokens=64)
+    fills = _fill(cache, 17)
+    q = torch.randn(new, G, hd, device="cuda", generator=torch.Generator(device="cuda").manual_seed(5)).half()
+    q[new // 2, 1, 77] = float("nan")
+    out, lse = torch.empty_like(q), torch.empty(new, G, device="cuda")
+    cache.attn(0, _batch([new], [kv]), q, out=out, lse=lse, logit_scale=0.1)
+    assert cache.status() == 0
+    assert torch.isnan(out[new // 2, 1]).all() and torch.isnan(lse[new // 2, 1])
+    for head in (0, 2, 3):
+        _check_attn(cache, fills, 0, q[:, head:head + 1], [new], [kv], None, out[:, head:head + 1], lse[:, head:head + 1],
+                    0.1, True, 0)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
 def test_example_runs(cuda, fmt):
     """The example: rotation, write, attention over prompts and a graph of single tokens."""
     import importlib.util
