@@ -62,7 +62,7 @@ template <int HD, int NT, int STAGES>
 struct FewSmem {
     unsigned char ring[kWarps][STAGES][Stage<HD>::Bytes];
     uint2 q[NT][HD / 16][32];                 // query fragments, one 8-byte word a lane
-    float up[8 * NT];                         // 2^exponent of each row
+    float mul[8 * NT];                        // each row's factor of the scores, in base 2
     float m[kWarps][8 * NT], l[kWarps][8 * NT];
     float o[4][8 * NT][HD + 4];               // + 4: rows on different banks
     unsigned scan[kWarps], found[3];
@@ -87,10 +87,10 @@ struct FewSmem {
 // sum w / vs.
 //
 // Measured: 16 sequences of 5693 to 32768 positions, one token each, 32 query
-// heads on 8 of 128 dimensions, e4m3: 119 us for 653 MB, 5.5 TB/s (84% of the
+// heads on 8 of 128 dimensions, e4m3: 118 us for 653 MB, 5.5 TB/s (84% of the
 // card's copy rate): memory bounds it, and what is left is the start of the
 // runs and their join.  With up to 32 rows (4 draft tokens, 32 query heads on 4
-// of 64 dimensions, int8; 48 sequences of 1296 to 9005) the 129 MB take 75 us:
+// of 64 dimensions, int8; 48 sequences of 1296 to 9005) the 129 MB take 73 us:
 // about 500 instructions of a warp for 16 positions, issued in half of the
 // cycles by the 16 warps that the registers of 32 rows' accumulators leave an
 // SM.  Copies go into a ring for each warp, without a barrier in the loop: loads
@@ -100,7 +100,9 @@ __global__ void __launch_bounds__(kThreads, CTAS) k_q8_attn_few(const __grid_con
 {
     constexpr int KS = HD / 16;               // k-steps of the scores, 32-bit code words of a K row in a lane
     constexpr int VW = HD / 32;               // code words of a V row in a lane
-    constexpr bool kQInRegs = NT * KS <= 8;
+    // what does not fit beside the accumulators is read from shared memory again
+    // for each tile (kept in registers it spills: draft tokens 73 -> 76 us)
+    constexpr bool kQInRegs = NT * KS <= 8, kMulInRegs = kQInRegs || CTAS == 1;
     extern __shared__ __align__(16) unsigned char smem_raw[];
     FewSmem<HD, NT, STAGES> &sm = *reinterpret_cast<FewSmem<HD, NT, STAGES> *>(smem_raw);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
@@ -173,17 +175,18 @@ __global__ void __launch_bounds__(kThreads, CTAS) k_q8_attn_few(const __grid_con
 
         // ---- the warp's ring: 16 positions a stage, copied a few stages ahead
         using St = Stage<HD>;
-        const uint32_t ring = (uint32_t)__cvta_generic_to_shared(sm.ring[warp]);
-        auto fetch = [&](int j0, int st) {
-            constexpr int kChunks = HD / 16, kRows = 32 / kChunks;       // 16-byte pieces of a row, rows at a time
-            const int r0 = lane / kChunks, pc = lane % kChunks * 16;
-            const uint32_t dk = ring + st * St::Bytes + r0 * St::KPitch + pc, dv = dk + 16 * St::KPitch;
-            const long long at = (long long)(j0 + r0) * HD + pc;
+        constexpr int kChunks = HD / 16, kRows = 32 / kChunks;           // 16-byte pieces of a row, rows at a time
+        const uint32_t ring = (uint32_t)__cvta_generic_to_shared(sm.ring[warp]) + lane / kChunks * St::KPitch + lane % kChunks * 16;
+        const uint8_t *kf, *vf;                // this lane's next pieces
+        auto fetch = [&](int st) {
+            const uint32_t dk = ring + st * St::Bytes, dv = dk + 16 * St::KPitch;
 #pragma unroll
             for (int r = 0; r < 16; r += kRows) {
-                copy_async16(dk + r * St::KPitch, kp + at + r * HD);
-                copy_async16(dv + r * St::VPitch, vp + at + r * HD);
+                copy_async16(dk + r * St::KPitch, kf + r * HD);
+                copy_async16(dv + r * St::VPitch, vf + r * HD);
             }
+            kf += kTile * HD;
+            vf += kTile * HD;
         };
         // dimension of code word i of a V row
         auto dim_of = [&](int i) { return HD == 64 ? 8 * g + 4 * i : 128 * (i / 4) + 16 * g + 4 * (i % 4); };
@@ -191,13 +194,15 @@ __global__ void __launch_bounds__(kThreads, CTAS) k_q8_attn_few(const __grid_con
         int j0 = u.start + k0 * kTile + 16 * warp;
         const int j_stop = min(u.end, u.start + k1 * kTile);
         int jf = j0;                           // next positions to fetch
+        kf = kp + (long long)(j0 + lane / kChunks) * HD + lane % kChunks * 16;
+        vf = vp + (long long)(j0 + lane / kChunks) * HD + lane % kChunks * 16;
         float ks[STAGES], vs[STAGES];          // scales of the stages in flight, oldest first
 #pragma unroll
         for (int i = 0; i < STAGES; i++) {
             ks[i] = 0.0f;
             vs[i] = 1.0f;
             if (jf < j_stop) {
-                fetch(jf, i);
+                fetch(i);
                 ks[i] = ksp[jf >> a.l.block_log2];
                 vs[i] = vsp[jf >> a.l.block_log2];
             }
@@ -227,7 +232,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) k_q8_attn_few(const __grid_con
             for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
             float down, up;
             row_scale(top, down, up);
-            if (lane == 0) sm.up[row] = up;
+            if (lane == 0) sm.mul[row] = a.scale * kLog2e * up;
 #pragma unroll
             for (int i = 0; i < E; i++) {
                 const int d = lane + 32 * i, s = d / 64 * 4 + d % 16 / 4;
@@ -243,7 +248,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) k_q8_attn_few(const __grid_con
 #pragma unroll
                 for (int s = 0; s < KS; s++) qr[n][s] = sm.q[n][s][lane];
         }
-        float mul[NT][2], m[NT][2], l[NT][2];
+        float mul[kMulInRegs ? NT : 1][2], m[NT][2], l[NT][2];
         // the positions that a row sees: kept with 8 rows, found again where a mask
         // asks for them with more, whose registers then hold two CTAs on an SM
         int hi[2], lo[2];
@@ -262,7 +267,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) k_q8_attn_few(const __grid_con
         for (int n = 0; n < NT; n++)
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                mul[n][i] = a.scale * kLog2e * sm.up[8 * n + 2 * c + i];
+                if (kMulInRegs) mul[kMulInRegs ? n : 0][i] = sm.mul[8 * n + 2 * c + i];
                 m[n][i] = kNone;
                 l[n][i] = 0.0f;
             }
@@ -314,14 +319,14 @@ __global__ void __launch_bounds__(kThreads, CTAS) k_q8_attn_few(const __grid_con
             }
 
             // ---- weights
-            const float lv = lg2(v_scale), iv = __frcp_rn(v_scale);
+            const float lv = lg2(v_scale), iv = rcp(v_scale);
             const bool all = j0 + 15 <= hi_min && j0 >= lo_max;     // nothing is masked
             bool over = false;
 #pragma unroll
             for (int n = 0; n < NT; n++)
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
-                    const float f = k_scale * mul[n][i];
+                    const float f = k_scale * (kMulInRegs ? mul[kMulInRegs ? n : 0][i] : sm.mul[8 * n + 2 * c + i]);
                     s[n][i] = fmaf(s[n][i], f, lv);
                     s[n][2 + i] = fmaf(s[n][2 + i], f, lv);
                     if (!all) {
@@ -400,7 +405,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) k_q8_attn_few(const __grid_con
                 }
             }
             __syncwarp();                      // all lanes have read the stage
-            if (jf < j_stop) fetch(jf, st);
+            if (jf < j_stop) fetch(st);
             copy_commit();
             jf += kTile;
             st = st + 1 == STAGES ? 0 : st + 1;

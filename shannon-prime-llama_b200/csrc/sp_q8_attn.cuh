@@ -65,6 +65,14 @@ __device__ __forceinline__ float lg2(float x)
     return y;
 }
 
+// 1 / x to the last place, for x whose reciprocal is a normal number.
+__device__ __forceinline__ float rcp(float x)
+{
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 // Four codes (bytes 0..3 of x) as fp16 pairs, lo = (0, 1) and hi = (2, 3),
 // exactly.
 //   int8: q + 128 placed in the low mantissa of 1024, then 1152 taken off:
