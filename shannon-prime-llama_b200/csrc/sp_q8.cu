@@ -220,7 +220,7 @@ __device__ __forceinline__ uint2 encode8(float (&x)[8])
 // Memory and the chain load, maximum, barrier, codes, store bound it: 33042
 // tokens of prompts in bf16 (8 heads of 128, blocks of 32, e4m3; 195 MB) take 39
 // us, 76% of the copy rate; 8192 in 32 bits (16 heads of 256, blocks of 128,
-// int8; 336 MB) 70 us, 74%.  With places and masks found anew for each pair and
+// int8; 336 MB) 63 us, 81%.  With places and masks found anew for each pair and
 // maxima joined by shuffles 47 and 77 us; one pair for each CTA, without the
 // next one's input on its way, 68 and 104 us.  Single tokens of 16 sequences
 // take 6.8 us, most of it the launch.
@@ -445,13 +445,15 @@ extern "C" int sp_cuda_q8_write_kv_tokens(sp_cuda_q8_cache_t *qc, int layer, con
     const long long units = each < all ? each : all;
     if (units > 0x7fffffff / 4) return sp_set_error(SP_ERR_ARG, "q8_write: %lld blocks in one call", units);
     a.slots = n * H;
-    // Pairs in turn where there are blocks enough to fill the SMs several times
-    // over: a step of single tokens wants a CTA for each instead.
-    long long in_turn = units * a.slots / (16ll * qc->sm_count);
+    const int threads = (int)(B * hd / 32);
+    // Pairs in turn where there are blocks enough to fill the SMs' threads more
+    // than twice over (prompts of the kernel's comment: 39 us for 6 in turn, 45 for
+    // 2; its 32-bit inputs: 63 us for 7, 66 for 2, 69 for 1): a step of single
+    // tokens wants a CTA for each instead.
+    long long in_turn = units * a.slots * threads / (2048ll * qc->sm_count);
     in_turn = in_turn < 1 ? 1 : in_turn > 16 ? 16 : in_turn;
     a.slots_each = (int)(in_turn < a.slots ? in_turn : a.slots);
     const dim3 grid((unsigned)units, (a.slots + a.slots_each - 1) / a.slots_each);
-    const int threads = (int)(B * hd / 32);
     cudaStream_t s = (cudaStream_t)qc->stream;
     return qc->format == SP_Q8_INT8 ? launch_write_of<SP_Q8_INT8>(a, dtype, hd, grid, threads, s)
                                     : launch_write_of<SP_Q8_E4M3>(a, dtype, hd, grid, threads, s);
