@@ -91,7 +91,7 @@ struct FewSmem {
 // card's copy rate): memory bounds it, and what is left is the start of the
 // runs and their join.  With up to 32 rows (4 draft tokens, 32 query heads on 4
 // of 64 dimensions, int8; 48 sequences of 1296 to 9005) the 129 MB take 73 us:
-// about 500 instructions of a warp for 16 positions, issued in half of the
+// about 470 instructions of a warp for 16 positions, issued in half of the
 // cycles by the 16 warps that the registers of 32 rows' accumulators leave an
 // SM.  Copies go into a ring for each warp, without a barrier in the loop: loads
 // straight into registers, a tile ahead, took 137 us and 86 us.

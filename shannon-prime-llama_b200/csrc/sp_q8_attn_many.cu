@@ -13,6 +13,19 @@
 // (8 rows of 16 bytes) that serves K as the K-major and V as the MN-major
 // operand.  One thread issues the products; while a softmax warpgroup works on
 // its 128 rows, the tensor cores work on the other 128.
+//
+// Measured: a causal prompt of 8192 tokens, 32 query heads on 8 of 128
+// dimensions, e4m3 and bf16, takes 705 us, 780 TFLOP/s (47% of the library's
+// plain product); chunks of 202 to 1021 tokens on up to 7570 positions, 16 query
+// heads on 2 of 256, int8, window 4096, 270 us, 685 TFLOP/s.  What bounds it is
+// the chain of a 128-row tile: scores, softmax (one row a thread, about 1950
+// cycles for 128 positions with two warps on each scheduler), store of the
+// weights (700), P V and the next scores (1400).  A tile of both halves takes
+// 3900 cycles, the products 2100 of them.  Tensor memory is full (two scores,
+// two outputs), so the next scores cannot be computed earlier: in halves of 64
+// columns, one of them ahead, the prompt took 994 us, since products of 64
+// columns cost 3/4 of those of 128.  The beginning and end of a unit (queries,
+// output) take about 12000 cycles, a tenth of the prompt's time.
 #include "sp_q8_attn.cuh"
 #include "sp_bulk.cuh"
 
@@ -830,7 +843,8 @@ out:
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
 }
 
-// Joins the parts of units that fell into several runs: block (i, y) the unit
+// Joins the parts of units that fell into several runs (a unit of 256 rows and
+// 128 dimensions leaves 133 KB a run, too much for the tail of one CTA): block (i, y) the unit
 // that began in run i, 16 of the head's dimensions, a thread for each row.
 template <typename T, int FMT, int HD>
 __global__ void __launch_bounds__(Shape<HD>::ROWS) k_q8_attn_join(const __grid_constant__ AttnArgs a)
