@@ -139,15 +139,17 @@ __device__ __forceinline__ F2 add2(F2 a, F2 b)
         : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
     return d;
 }
-// 2^x for x >= -126 (below: 2^-126) without the special-function unit: the
+// 2^x for x in [-126, 126] (below: 2^-126; above, and for NaN: 2^126, which the
+// test for too small a maximum sees) without the special-function unit: the
 // nearest whole number n by adding and taking off 1.5 * 2^23, whose low bits
-// then are n and go to the exponent; 2^(x - n) by the polynomial of degree 4
-// with the least largest relative error on [-1/2, 1/2], 2.7e-6 (Remez exchange).
+// then are n and go to the exponent, which would wrap outside those limits;
+// 2^(x - n) by the polynomial of degree 4 with the least largest relative error
+// on [-1/2, 1/2], 2.7e-6 (Remez exchange).
 __device__ __forceinline__ F2 exp2_poly(F2 x)
 {
     constexpr float kRound = 12582912.0f;
-    x.x = fmaxf(x.x, -126.0f);
-    x.y = fmaxf(x.y, -126.0f);
+    x.x = fmaxf(fminf(x.x, 126.0f), -126.0f);
+    x.y = fmaxf(fminf(x.y, 126.0f), -126.0f);
     const F2 t = add2(x, {kRound, kRound}), n = add2(t, {-kRound, -kRound}), r = fma2(n, {-1.0f, -1.0f}, x);
     F2 p = fma2({0x1.3997d6p-7f, 0x1.3997d6p-7f}, r, {0x1.ca1444p-5f, 0x1.ca1444p-5f});
     p = fma2(p, r, {0x1.ec06dap-3f, 0x1.ec06dap-3f});
@@ -284,12 +286,12 @@ struct Walk {
     }
 };
 
-// Which pairs of weights take the polynomial: one in four at head_dim 64, whose
+// Which pairs of weights take the polynomial: one in eight at head_dim 64, whose
 // products are short, so that the special-function unit bounds a tile (a causal
-// prompt of 8192 with 32 heads on 8: 553 us against 572 without; at 128 it makes
-// no difference, 707 and 710, and half of the pairs take 735).
+// prompt of 8192 with 32 heads on 8: 559 us; one in four 561, none 567; at 128
+// one in four makes no difference, 707 and 710, and half of the pairs take 735).
 template <int HD>
-__host__ __device__ constexpr bool kPoly(int j) { return HD == 64 && j % 4 == 3; }
+__host__ __device__ constexpr bool kPoly(int j) { return HD == 64 && j % 8 == 3; }
 
 template <typename T, int FMT, int HD>
 __global__ void __launch_bounds__(Shape<HD>::Threads, 1) k_q8_attn_many(const __grid_constant__ AttnArgs a)

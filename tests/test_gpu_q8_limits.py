@@ -1,0 +1,107 @@
+"""The 8-bit tier on the GPU at the ends of what it accepts.  Bounds are those
+of test_gpu_q8.py."""
+import numpy as np
+import pytest
+import torch
+
+import q8_ref as R
+import spb200
+from test_gpu_q8 import _batch, _check_attn, _fill
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------- logits that rise late and far --
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("fmt,dtype", [("int8", "f16"), ("e4m3", "bf16")])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("new", [2, 40])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_attn_one_key_far_above(cuda, hd, fmt, dtype, causal, new, zeros):
+    """Ordinary logits, then one key 2^100 to 2^500 times the others' weight, at
+    each position mod 32 (a sequence for each) past the first tiles; `zeros`: after
+    values whose blocks have the smallest scale, as a write of zeros leaves them."""
+    H, G, B, n, seqs = 1, 4, 64, 600, 32
+    cache = spb200.Q8Cache(hd, 1, H, n, n_seqs=seqs, fmt=fmt, block_tokens=B)
+    kc, ks, vc, vs = _fill(cache, 31)
+    g = torch.Generator().manual_seed(8)
+    u = torch.randint(0, 2, (hd,), generator=g).float() * 2 - 1
+    kc.copy_(R.code(torch.randn(kc.shape, generator=g) * 2.5, fmt).view(kc.shape))
+    ks.fill_(2.0 ** -7)
+    for i in range(seqs):
+        kc[0, i, 0, 256 + 32 * (i % 8) + i] = R.code(112.0 * u, fmt)
+    if zeros:
+        vc[:, :, :, :256] = 0
+        vs[:, :, :, :256 // B] = 2.0 ** -40
+    for which, c, s in ((0, kc, ks), (1, vc, vs)):
+        cache.slab(which).view(torch.uint8).copy_(c)
+        cache.scales(which).copy_(s)
+    q = u + 0.25 * torch.randn(seqs * new, G, hd, generator=g)
+    q = q.to(R.DTYPES[dtype]).cuda()
+    out, lse = torch.empty_like(q), torch.empty(seqs * new, G, device="cuda")
+    b = _batch([new] * seqs, [n] * seqs)
+    for rise in (100, 130, 200, 256, 300, 500):
+        scale = rise * np.log(2.0) / (112.0 * hd / 128)
+        cache.attn(0, b, q, out=out, lse=lse, logit_scale=scale, causal=causal)
+        assert cache.status() == 0
+        _check_attn(cache, (kc, ks, vc, vs), 0, q, [new] * seqs, [n] * seqs, None, out, lse, scale, causal, 0)
+
+
+@pytest.mark.parametrize("hd", [64, 256])
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("new", [1, 100])
+def test_attn_scales_far_apart_other_dims(cuda, hd, fmt, new):
+    """Blocks of V whose scales span 2^-40 .. 2^12, one of zeros: every weight counts in the sum."""
+    B, n = 16, 160
+    cache = spb200.Q8Cache(hd, 1, 1, n, fmt=fmt, block_tokens=B)
+    fills = _fill(cache, 5)
+    fills[1][0, 0, 0, :10] = 0.02
+    fills[3][0, 0, 0, :10] = torch.tensor([2.0 ** -12, 0.03, 0.02, 0.05, 0.01, 2.0 ** -40, 0.03, 0.02, 2.0 ** -20, 2.0 ** 12])
+    fills[2][0, 0, 0, 5 * B:6 * B] = 0
+    for c in (0, 1):
+        cache.slab(c).view(torch.uint8).copy_(fills[2 * c])
+        cache.scales(c).copy_(fills[2 * c + 1])
+    for end in (B, 5 * B + 3, 6 * B, 9 * B, n):
+        for scale in (0.0, 0.05, 2.0):
+            m = min(new, end)
+            q = torch.randn(m, 4, hd, device="cuda", generator=torch.Generator(device="cuda").manual_seed(end)).half()
+            out, lse = torch.empty_like(q), torch.empty(m, 4, device="cuda")
+            cache.attn(0, _batch([m], [end]), q, out=out, lse=lse, logit_scale=scale)
+            _check_attn(cache, fills, 0, q, [m], [end], None, out, lse, scale, True, 0)
+
+
+@pytest.mark.parametrize("hd", [64, 256])
+@pytest.mark.parametrize("new", [1, 100])
+def test_attn_large_and_small_queries_other_dims(cuda, hd, new):
+    """bf16 queries far outside fp16's range, rows of zeros, logits far apart along the sequence."""
+    n = 700
+    cache = spb200.Q8Cache(hd, 1, 1, n, fmt="int8", block_tokens=64)
+    fills = _fill(cache, 9)
+    q = torch.randn(new, 4, hd, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))
+    q[:, 0] *= 1e20
+    q[:, 1] *= 1e-20
+    q[:, 2] = 0
+    q = q.to(torch.bfloat16)
+    out, lse = torch.empty_like(q), torch.empty(new, 4, device="cuda")
+    for head, scale in ((0, 3e-21), (1, 3e19), (2, 1.0), (3, 20.0)):
+        cache.attn(0, _batch([new], [n]), q, out=out, lse=lse, logit_scale=scale)
+        _check_attn(cache, fills, 0, q[:, head:head + 1], [new], [n], None, out[:, head:head + 1], lse[:, head:head + 1],
+                    scale, True, 0)
+
+
+@pytest.mark.parametrize("hd", [64, 256])
+@pytest.mark.parametrize("new,kv", [(3, 90), (100, 700)])
+def test_attn_nan_queries_other_dims(cuda, hd, new, kv):
+    """A query row with a NaN has NaN for its output and lse; the others are as they should be."""
+    cache = spb200.Q8Cache(hd, 1, 1, kv, fmt="e4m3", block_tokens=64)
+    fills = _fill(cache, 17)
+    q = torch.randn(new, 4, hd, device="cuda", generator=torch.Generator(device="cuda").manual_seed(5)).half()
+    q[new // 2, 1, 33] = float("nan")
+    out, lse = torch.empty_like(q), torch.empty(new, 4, device="cuda")
+    cache.attn(0, _batch([new], [kv]), q, out=out, lse=lse, logit_scale=0.1)
+    assert cache.status() == 0
+    assert torch.isnan(out[new // 2, 1]).all() and torch.isnan(lse[new // 2, 1])
+    for head in (0, 2, 3):
+        _check_attn(cache, fills, 0, q[:, head:head + 1], [new], [kv], None, out[:, head:head + 1], lse[:, head:head + 1],
+                    0.1, True, 0)
