@@ -34,9 +34,10 @@ def _rows(t, heads, head_dim: int, what: str) -> int:
         if t.is_contiguous():
             return 0
         s = t.stride()
-        if s[2] == 1 and (sh[1] == 1 or s[1] == head_dim):
+        # tokens that share memory (an expanded tensor's, whose stride is 0) have less than the shape says
+        if s[2] == 1 and (sh[1] == 1 or s[1] == head_dim) and s[0] >= sh[1] * head_dim:
             return s[0]
-    raise ValueError(f"{what}: a token's heads must lie together in device memory")
+    raise ValueError(f"{what}: a token's heads must lie together in device memory, and tokens apart from one another")
 
 
 class RopeAxes:

@@ -1,0 +1,82 @@
+"""What the 8-bit tier's binding refuses before anything is launched.  No GPU:
+tensors in main memory stand in for tensors of a card."""
+import pytest
+import torch
+
+
+class OnCard:
+    """A tensor that says it lies on card 0; nothing is launched on it."""
+
+    is_cuda = True
+
+    def __init__(self, t, device=0):
+        self.t, self.device = t, torch.device("cuda", device)
+
+    def __getattr__(self, name):
+        return getattr(self.t, name)
+
+    def get_device(self):
+        return self.device.index
+
+
+def _cache(hd=64, heads=2):
+    """A Q8Cache that has its shape and no memory."""
+    import spb200
+    c = object.__new__(spb200.Q8Cache)
+    c.qc = spb200.SpQ8Cache()
+    c.head_dim, c.n_heads_kv, c.fmt, c.stream = hd, heads, "int8", None
+    c._ref = None
+
+    def launched(*a):
+        raise AssertionError("the call reached the library")
+    c._write = c._read = c._attn = launched
+    return c
+
+
+def _batch(n_tokens):
+    import spb200
+    b = object.__new__(spb200.Q8Batch)
+    b._keep, b.n_tokens, b.ref, b.device = (), n_tokens, None, 0
+    return b
+
+
+def _rope():
+    import spb200
+    r = spb200.RopeAxes(64, [32])
+
+    def launched(*a):
+        raise AssertionError("the call reached the library")
+    r._call = launched
+    return r, OnCard(torch.zeros(1, 5, dtype=torch.int32))
+
+
+def _one(heads=2, dtype=torch.float16):
+    """Five tokens that are one token's memory."""
+    return OnCard(torch.zeros(1, heads, 64, dtype=dtype).expand(5, heads, 64))
+
+
+def _all(heads=2, dtype=torch.float16):
+    return OnCard(torch.zeros(5, heads, 64, dtype=dtype))
+
+
+def test_tokens_that_share_memory_are_refused(built_lib):
+    """A tensor expanded over its tokens has less memory than its shape says."""
+    rope, pos = _rope()
+    cache, batch = _cache(), _batch(5)
+    overlapping = OnCard(torch.zeros(600, dtype=torch.float16).as_strided((5, 2, 64), (64, 64, 1)))
+    for bad in (_one(), overlapping):
+        for call in (lambda: rope.apply(pos, bad, None, q_out=_all()), lambda: rope.apply(pos, None, bad, k_out=_all()),
+                     lambda: rope.apply(pos, _all(), None, q_out=bad), lambda: rope.apply(pos, None, _all(), k_out=bad),
+                     lambda: cache.write_kv_tokens(0, batch, bad, None), lambda: cache.write_kv_tokens(0, batch, None, bad),
+                     lambda: cache.write_kv_tokens(0, batch, bad, bad), lambda: cache.attn(0, batch, bad, out=_all()),
+                     lambda: cache.attn(0, batch, _all(), out=bad), lambda: cache.read_kv_tokens(0, 0, 0, 0, bad)):
+            with pytest.raises(ValueError):
+                call()
+
+
+def test_one_token_may_be_expanded(built_lib):
+    """One token has all the memory it needs, whatever its stride."""
+    import spb200.q8 as q8
+    assert q8._rows(OnCard(torch.zeros(1, 1, 64).expand(1, 1, 64)), 1, 64, "x") == 0
+    fused = OnCard(torch.zeros(5, 6, 64)[:, 2:4])
+    assert q8._rows(fused, 2, 64, "x") == 6 * 64
