@@ -607,6 +607,9 @@ extern "C" int sp_cuda_q8_attn(const sp_cuda_q8_cache_t *qc, int layer, const sp
         return sp_set_error(SP_ERR_ARG, "q8_attn: %d query heads for %d KV heads", n_q_heads, H);
     if (!isfinite(logit_scale)) return sp_set_error(SP_ERR_ARG, "q8_attn: logit scale %g", (double)logit_scale);
     if (window < 0 || (window && !causal)) return sp_set_error(SP_ERR_ARG, "q8_attn: window %d", window);
+    // past the cache's length a window hides nothing; so bounded, position - window
+    // stays in 32 bits for tokens before the first position too
+    if (window > qc->max_seq_len) window = qc->max_seq_len;
     if (q_stride == 0) q_stride = (long long)n_q_heads * hd;
     if (out_stride == 0) out_stride = (long long)n_q_heads * hd;
     if (q_stride < (long long)n_q_heads * hd || out_stride < (long long)n_q_heads * hd)

@@ -6,7 +6,7 @@ import torch
 
 import q8_ref as R
 import spb200
-from test_gpu_q8 import _batch, _check_attn, _fill
+from test_gpu_q8 import _batch, _check_attn, _fill, _run_attn
 
 pytestmark = pytest.mark.gpu
 
@@ -105,3 +105,13 @@ def test_attn_nan_queries_other_dims(cuda, hd, new, kv):
     for head in (0, 2, 3):
         _check_attn(cache, fills, 0, q[:, head:head + 1], [new], [kv], None, out[:, head:head + 1], lse[:, head:head + 1],
                     0.1, True, 0)
+
+
+# -------------------------------------------------------- windows and tokens --
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 30, 257, 256])
+@pytest.mark.parametrize("new,kv", [([5, 2, 1], [2, 2, 0]), ([90, 3, 60], [20, 250, 256])])
+def test_attn_windows_past_the_cache(cuda, hd, window, new, kv):
+    """The widest windows, with tokens before the first position."""
+    _run_attn(hd, 1, 4, 16, "int8", "f16", new, kv, window=window, max_seq=256)
