@@ -27,6 +27,7 @@
 // columns cost 3/4 of those of 128.  The beginning and end of a unit (queries,
 // output) take about 12000 cycles, a tenth of the prompt's time.
 #include "sp_q8_attn.cuh"
+#include "sp_q8_runs.h"
 #include "sp_bulk.cuh"
 
 #include <atomic>
@@ -59,10 +60,9 @@ struct ManySmem {
     unsigned char k[2][Shape<HD>::StageB], v[2][Shape<HD>::StageB];
     unsigned long long q_full[2], k_full[2], k_free[2], v_full[2], v_free[2], s_full[2], p_full[2], pv_done[2], end;
     float4 scales[4][Shape<HD>::BN / 16];              // of four tiles in turn: K scale, log2 of V's, 1 / V's
-    unsigned scan[32];
-    unsigned tiles[256];                               // of one head of each entry of a chunk, then their prefix
+    unsigned long long tiles[256], total;              // of each entry of a chunk; of the entries so far
+    unsigned long long found_t;
     int found;
-    unsigned found_t;
     uint32_t tmem;
     int abort;
 };
@@ -71,7 +71,7 @@ struct ManySmem {
 // the run in which the unit begins.
 struct Split {
     int valid, q0, row0, rows, head;
-    unsigned unit_t, run0, run1;
+    unsigned run0, run1;
 };
 
 // --- tensor core and tensor memory --------------------------------------
@@ -262,15 +262,15 @@ template <int HD>
 struct Walk {
     Entry e;
     int ei, qt, n_qt, head;
-    unsigned t, t_end, unit_t;      // next tile, end of the run, first tile of the unit
+    unsigned t, t_end, unit_t;      // next tile, end of the run, first tile of the unit: their low 32 bits
     Rows r;
-    __device__ __forceinline__ bool more() const { return t < t_end; }
+    __device__ __forceinline__ bool more() const { return apart(t_end, t) > 0; }
     __device__ __forceinline__ int k0() const { return t - unit_t; }
     __device__ __forceinline__ int k1() const { return min((unsigned)r.tiles, t_end - unit_t); }
     __device__ __forceinline__ void next(const AttnArgs &a)
     {
         t = unit_t + k1();
-        if (t >= t_end) return;
+        if (!more()) return;
         unit_t += r.tiles;
         if (++qt == n_qt) {
             qt = 0;
@@ -308,8 +308,8 @@ __global__ void __launch_bounds__(Shape<HD>::Threads, 1) k_q8_attn_many(const __
 
     // ---- this CTA's run: tiles of one head of each entry (a warp for an entry, a lane for
     // a tile of rows), their sum, and the entry in which the run begins
-    Runs runs;
-    unsigned before = 0;
+    LongRuns runs;
+    unsigned long long before = 0;
     for (int pass = 0; pass < 2; pass++) {
         before = 0;
         for (int base = 0; base < a.b.n_seqs; base += 256) {
@@ -317,7 +317,7 @@ __global__ void __launch_bounds__(Shape<HD>::Threads, 1) k_q8_attn_many(const __
             for (int i = warp; i < n; i += kWarps) {
                 const Entry e = entry(a.b, base + i);
                 const int nq = row_tiles<HD>(a, e);
-                unsigned sum = 0;
+                unsigned long long sum = 0;
                 for (int q = lane; q < nq; q += 32) sum += rows_of<HD>(a, e, q).tiles;
 #pragma unroll
                 for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
@@ -326,15 +326,15 @@ __global__ void __launch_bounds__(Shape<HD>::Threads, 1) k_q8_attn_many(const __
             __syncthreads();
             if (warp == 0) {
                 for (int i = 0; i < n; i += 32) {
-                    const unsigned x = i + lane < n ? sm.tiles[i + lane] : 0;
-                    unsigned upto = x;
+                    const unsigned long long x = i + lane < n ? sm.tiles[i + lane] : 0;
+                    unsigned long long upto = x;
 #pragma unroll
                     for (int d = 1; d < 32; d <<= 1) {
-                        const unsigned o = __shfl_up_sync(0xffffffffu, upto, d);
+                        const unsigned long long o = __shfl_up_sync(0xffffffffu, upto, d);
                         if (lane >= d) upto += o;
                     }
                     if (pass) {
-                        const unsigned t = run_begin(runs, blockIdx.x);
+                        const unsigned long long t = run_begin(runs, blockIdx.x);
                         if (t >= before + upto - x && t < before + upto) {
                             sm.found = base + i + lane;
                             sm.found_t = before + upto - x;
@@ -342,38 +342,38 @@ __global__ void __launch_bounds__(Shape<HD>::Threads, 1) k_q8_attn_many(const __
                     }
                     before += __shfl_sync(0xffffffffu, upto, 31);
                 }
-                if (lane == 0) sm.scan[0] = before;
+                if (lane == 0) sm.total = before;
             }
             __syncthreads();
-            before = sm.scan[0];
+            before = sm.total;
             __syncthreads();
         }
         if (pass == 0) {
-            runs = runs_of(before, gridDim.x);
+            runs = long_runs_of(before, gridDim.x);
             if (blockIdx.x >= runs.n) return;
         }
     }
     Walk<HD> w;
-    w.t = run_begin(runs, blockIdx.x);
-    w.t_end = run_begin(runs, blockIdx.x + 1);
+    w.t = (unsigned)run_begin(runs, blockIdx.x);
+    w.t_end = (unsigned)run_begin(runs, blockIdx.x + 1);
     w.ei = sm.found;
     w.e = entry(a.b, w.ei);
     w.n_qt = row_tiles<HD>(a, w.e);
     {
         // the head, then the tile of rows, in which the run begins
-        unsigned each = 0;
+        unsigned long long each = 0;
         for (int q = lane; q < w.n_qt; q += 32) each += rows_of<HD>(a, w.e, q).tiles;
 #pragma unroll
         for (int d = 16; d; d >>= 1) each += __shfl_xor_sync(0xffffffffu, each, d);
-        const unsigned in = w.t - sm.found_t;
-        w.head = in / each;
-        const unsigned off = in - w.head * each;
-        unsigned pre = 0;
+        const unsigned long long in = run_begin(runs, blockIdx.x) - sm.found_t;
+        w.head = (int)(in / each);
+        const unsigned long long off = in - w.head * each;
+        unsigned long long pre = 0;
         w.qt = 0;
         w.unit_t = 0;
         for (int base = 0; base < w.n_qt; base += 32) {
             const unsigned x = base + lane < w.n_qt ? rows_of<HD>(a, w.e, base + lane).tiles : 0;
-            unsigned upto = x;
+            unsigned upto = x;               // of 32 tiles of rows, with at most 2^24 tiles of positions each
 #pragma unroll
             for (int d = 1; d < 32; d <<= 1) {
                 const unsigned o = __shfl_up_sync(0xffffffffu, upto, d);
@@ -383,7 +383,7 @@ __global__ void __launch_bounds__(Shape<HD>::Threads, 1) k_q8_attn_many(const __
             if (who) {
                 const int src = __ffs(who) - 1;
                 w.qt = base + src;
-                w.unit_t = w.t - (off - (pre + __shfl_sync(0xffffffffu, upto - x, src)));
+                w.unit_t = w.t - (unsigned)(off - (pre + __shfl_sync(0xffffffffu, upto - x, src)));
             }
             pre += __shfl_sync(0xffffffffu, upto, 31);
         }
@@ -682,7 +682,7 @@ __global__ void __launch_bounds__(Shape<HD>::Threads, 1) k_q8_attn_many(const __
                 if (real && a.lse) a.lse[(long long)tok * a.n_q_heads + qh] = l == 0.0f ? -INFINITY : kLn2 * (m + lg2(l));
             } else {
                 // rows side by side, so that a warp's stores are contiguous
-                float *part = a.partials + (long long)(2 * blockIdx.x + (w.unit_t >= run_begin(runs, blockIdx.x))) * S::SlotFloats;
+                float *part = a.partials + (long long)(2 * blockIdx.x + (apart(w.unit_t, (unsigned)run_begin(runs, blockIdx.x)) >= 0)) * S::SlotFloats;
                 const int prow = 128 * i + r;
 #pragma unroll 1
                 for (int c = 0; c < HD; c += 32) {
@@ -699,8 +699,9 @@ __global__ void __launch_bounds__(Shape<HD>::Threads, 1) k_q8_attn_many(const __
                 }
                 if (real) __stcg(reinterpret_cast<float2 *>(part + S::ROWS * HD) + prow, make_float2(m, l));
                 if (tid == 0 && k0 == 0) {
-                    const unsigned last = w.unit_t + w.r.tiles - 1;
-                    *splits = {1, w.e.q0, w.r.row0, w.r.rows, w.head, w.unit_t, (unsigned)blockIdx.x, run_of_tile(runs, last)};
+                    const unsigned long long begin_t = run_begin(runs, blockIdx.x);
+                    const unsigned long long last = begin_t + apart(w.unit_t, (unsigned)begin_t) + w.r.tiles - 1;
+                    *splits = {1, w.e.q0, w.r.row0, w.r.rows, w.head, (unsigned)blockIdx.x, run_of_tile(runs, last)};
                 }
             }
             fence_before();

@@ -80,3 +80,15 @@ def test_one_token_may_be_expanded(built_lib):
     assert q8._rows(OnCard(torch.zeros(1, 1, 64).expand(1, 1, 64)), 1, 64, "x") == 0
     fused = OnCard(torch.zeros(5, 6, 64)[:, 2:4])
     assert q8._rows(fused, 2, 64, "x") == 6 * 64
+
+
+def test_runs_of_more_tiles_than_32_bits_count(tmp_path):
+    """The many-row attention's cut into runs (tests/c/q8_runs_check.cpp)."""
+    import subprocess
+
+    from conftest import PKG, ROOT, load_build_module
+    b = load_build_module()
+    exe = tmp_path / "q8_runs_check"
+    subprocess.run([b.HOST_CXX, "-O1", "-std=c++17", "-Wall", "-Werror", f"-I{PKG / 'csrc'}",
+                    str(ROOT / "tests" / "c" / "q8_runs_check.cpp"), "-o", str(exe)], check=True)
+    assert subprocess.run([str(exe)], capture_output=True, text=True).stdout == "ok\n"
