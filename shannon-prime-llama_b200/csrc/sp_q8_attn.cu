@@ -619,6 +619,9 @@ extern "C" int sp_cuda_q8_attn(const sp_cuda_q8_cache_t *qc, int layer, const sp
     if (((uintptr_t)d_q | (uintptr_t)d_out | (uintptr_t)(q_stride * 2) | (uintptr_t)(out_stride * 2)) % 16 || (uintptr_t)d_lse % 4)
         return sp_set_error(SP_ERR_ARG, "q8_attn: pointers and strides must be multiples of 16 bytes");
     const int G = n_q_heads / H;
+    // rows of an entry are counted in 32 bits; a tensor of so many has 275 GB
+    if ((long long)(batch->max_new < batch->n_tokens ? batch->max_new : batch->n_tokens) * G > 0x7fffffff)
+        return sp_set_error(SP_ERR_ARG, "q8_attn: %d tokens of %d query heads for a KV head in one entry", batch->max_new, G);
     AttnArgs a = {q8::layer_of(qc, layer), q8::batch_of(qc, batch), d_q, d_out, d_lse, q_stride, out_stride,
                   n_q_heads, G, logit_scale, causal, window, 0, (unsigned int *)qc->d_attn_ws,
                   (float *)((char *)qc->d_attn_ws + kCounterBytes + q8::split_bytes(qc->sm_count))};

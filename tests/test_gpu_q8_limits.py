@@ -115,3 +115,15 @@ def test_attn_nan_queries_other_dims(cuda, hd, new, kv):
 def test_attn_windows_past_the_cache(cuda, hd, window, new, kv):
     """The widest windows, with tokens before the first position."""
     _run_attn(hd, 1, 4, 16, "int8", "f16", new, kv, window=window, max_seq=256)
+
+
+def test_attn_rows_past_32_bits_are_refused(cuda):
+    """Entries that may have 2^31 rows; a loose bound on an entry's tokens is no such claim."""
+    cache = spb200.Q8Cache(64, 1, 1, 256)
+    q = torch.randn(4, 128, 64, device="cuda", dtype=torch.float16)
+    p, call = q.data_ptr(), spb200.lib().sp_cuda_q8_attn
+    for tokens, most, rc in ((2 ** 30, 2 ** 30, spb200.SP_ERR_ARG), (2 ** 24, 2 ** 31 - 1, spb200.SP_ERR_ARG), (4, 2 ** 31 - 1, 0)):
+        b = spb200.Q8Batch(torch.tensor([0, 4], dtype=torch.int32, device="cuda"), torch.tensor([9], dtype=torch.int32, device="cuda"),
+                           tokens, most, 256)
+        assert call(cache._ref, 0, b.ref, p, 0, 128, 1, 1.0, 1, 0, p, 0, None, None) == rc, (tokens, most)
+    assert cache.status() == 0
