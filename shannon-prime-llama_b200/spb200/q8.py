@@ -1,6 +1,8 @@
 """Python mirror of the 8-bit cache (shannon_prime_q8.h): rotary positions
 with several axes, the quantising write, the read back and attention.  Every
-method calls straight into the C-ABI; device buffers are torch CUDA tensors."""
+method calls straight into the C-ABI; device buffers are torch CUDA tensors.
+As everywhere in torch, tensors given to a call on another stream than the one
+they were made on have to be ready there and to live until it has run."""
 from __future__ import annotations
 
 import ctypes as C
@@ -40,6 +42,22 @@ def _rows(t, heads, head_dim: int, what: str) -> int:
     raise ValueError(f"{what}: a token's heads must lie together in device memory, and tokens apart from one another")
 
 
+def _output(t, stream):
+    """An output like t, to be written on `stream` (None: the default stream).
+    Its memory is that stream's, so that whoever had it before, there, is done
+    with it, and goes back to it only after the current stream's work as well:
+    the output may be dropped while either still runs."""
+    import torch
+    now = torch.cuda.current_stream(t.device)
+    at = _stream_ptr(stream)
+    if now.cuda_stream == at:
+        return torch.empty(t.shape, dtype=t.dtype, device=t.device)
+    with torch.cuda.stream(torch.cuda.ExternalStream(at, t.device) if at else torch.cuda.default_stream(t.device)):
+        out = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+    out.record_stream(now)
+    return out
+
+
 class RopeAxes:
     """A rotation plan: `sections` pairs for each axis (together rot_dim / 2)."""
 
@@ -68,14 +86,14 @@ class RopeAxes:
         qp = qs = hq = qo = qos = kp = ks = hk = ko = kos = 0
         if q is not None:
             if q_out is None:
-                q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+                q_out = _output(q, stream)
             qs, qos, hq = _rows(q, None, hd, "q"), _rows(q_out, q.shape[1], hd, "q_out"), q.shape[1]
             qp, qo = q.data_ptr(), q_out.data_ptr()
             if q_out.dtype is not q.dtype or q_out.shape[0] != n:
                 raise ValueError("q and its output must have one type and number of tokens")
         if k is not None:
             if k_out is None:
-                k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+                k_out = _output(k, stream)
             ks, kos, hk = _rows(k, None, hd, "k"), _rows(k_out, k.shape[1], hd, "k_out"), k.shape[1]
             kp, ko = k.data_ptr(), k_out.data_ptr()
             if k_out.dtype is not k.dtype or k_out.shape[0] != n or k.shape[0] != n or k.dtype is not t.dtype:
@@ -179,8 +197,7 @@ class Q8Cache:
         given); lse: fp32 [n_tokens][n_q_heads] or None.  Returns out."""
         n, hq, hd = *q.shape[:2], self.head_dim
         if out is None:
-            import torch
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            out = _output(q, stream)
         qs, os = _rows(q, None, hd, "q"), _rows(out, hq, hd, "out")
         if n != batch.n_tokens or out.shape[0] != n or out.dtype is not q.dtype:
             raise ValueError(f"q and out must have one type and the batch's {batch.n_tokens} tokens")

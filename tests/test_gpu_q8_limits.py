@@ -127,3 +127,43 @@ def test_attn_rows_past_32_bits_are_refused(cuda):
                            tokens, most, 256)
         assert call(cache._ref, 0, b.ref, p, 0, 128, 1, 1.0, 1, 0, p, 0, None, None) == rc, (tokens, most)
     assert cache.status() == 0
+
+
+# ------------------------------------------------------------------- streams --
+
+@pytest.mark.parametrize("which", ["rope", "attn"])
+def test_new_outputs_are_memory_of_their_stream(cuda, which):
+    """An output that a call allocates is written on the call's stream: it is neither
+    memory that the current stream may still be using nor given out again while
+    either stream is busy with it."""
+    T, hd = 37, 64
+    x = torch.randn(T, 3, hd, device="cuda", dtype=torch.float16)
+    pos = torch.zeros(1, T, dtype=torch.int32, device="cuda")
+    rope, cache = spb200.RopeAxes(hd, [32]), spb200.Q8Cache(hd, 1, 3, 128)
+    batch = _batch([T], [T])
+
+    def call(**kw):
+        return rope.apply(pos, x, None, **kw)[0] if which == "rope" else cache.attn(0, batch, x, **kw)
+    torch.cuda.synchronize()
+    side, other = torch.cuda.Stream(), torch.cuda.Stream()
+    for stream, current in ((side, torch.cuda.default_stream()), (side, other), (None, other)):
+        with torch.cuda.stream(current):
+            old = torch.empty_like(x)
+            at = old.data_ptr()
+            del old
+            y = call(stream=stream)                 # not what the current stream has just given back
+            assert y.data_ptr() != at
+            at = y.data_ptr()
+            del y
+            z = torch.empty_like(x)                 # nor is it the current stream's to give out
+            assert z.data_ptr() != at
+            y = call(stream=stream)
+            current.wait_stream(stream or torch.cuda.default_stream())
+            at = y.data_ptr()
+            torch.cuda._sleep(20000000)             # about 10 ms
+            w = y.clone()
+            del y
+            y = call(stream=stream)                 # the copy of the last one has not run yet
+            assert y.data_ptr() != at
+            torch.cuda.synchronize()
+            assert torch.equal(w, y)
