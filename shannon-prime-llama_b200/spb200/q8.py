@@ -27,19 +27,20 @@ def _dtype(t) -> int:
     return code
 
 
-def _rows(t, heads, head_dim: int, what: str) -> int:
-    """The token stride of t [n_tokens][heads][head_dim] (0: dense), whose rows lie together."""
+def _rows(t, heads, head_dim: int, what: str, device: int = 0) -> int:
+    """The token stride of t [n_tokens][heads][head_dim] (0: dense), whose rows lie
+    together in memory of `device`."""
     sh = t.shape
     if len(sh) != 3 or sh[2] != head_dim or (heads is not None and sh[1] != heads):
         raise ValueError(f"{what}: shape {tuple(sh)}, not [tokens][{heads or 'heads'}][{head_dim}]")
-    if t.is_cuda:
+    if t.get_device() == device:
         if t.is_contiguous():
             return 0
         s = t.stride()
         # tokens that share memory (an expanded tensor's, whose stride is 0) have less than the shape says
         if s[2] == 1 and (sh[1] == 1 or s[1] == head_dim) and s[0] >= sh[1] * head_dim:
             return s[0]
-    raise ValueError(f"{what}: a token's heads must lie together in device memory, and tokens apart from one another")
+    raise ValueError(f"{what}: a token's heads must lie together in memory of device {device}, and tokens apart from one another")
 
 
 def _output(t, stream):
@@ -71,32 +72,37 @@ class RopeAxes:
         check(lib().sp_rope_axes_init(C.byref(self.plan), head_dim, rot_dim, _PAIRINGS[pairing], len(sections),
                                       (C.c_int * len(sections))(*sections), flags, theta, ff), "sp_rope_axes_init")
         self.head_dim, self.n_axes = head_dim, len(sections)
+        import torch
         self._ref, self._call = C.byref(self.plan), lib().sp_cuda_rope_axes
+        self._int32, self._device = torch.int32, torch.cuda.current_device      # a step's call is host time
 
     def apply(self, pos, q=None, k=None, q_out=None, k_out=None, inverse: bool = False, stream=None):
         """Rotates q and k ([tokens][heads][head_dim] CUDA tensors; either may be
         None) at positions pos (int32 [axes][tokens]).  The outputs are new
         tensors unless given; an output may be its input.  Returns both."""
-        import torch
         t = k if q is None else q
-        n = 0 if t is None else t.shape[0]
-        if pos.dtype is not torch.int32 or pos.shape != (self.n_axes, n) or not (pos.is_cuda and pos.is_contiguous()):
+        n, dev = 0 if t is None else t.shape[0], pos.get_device()
+        if pos.dtype is not self._int32 or pos.shape != (self.n_axes, n) or dev < 0 or not pos.is_contiguous():
             raise ValueError(f"pos must be a contiguous int32 CUDA tensor [{self.n_axes}][{n}]")
+        if dev != self._device():
+            raise ValueError(f"pos is on device {dev}, the current device is {self._device()}")
         hd = self.head_dim
         qp = qs = hq = qo = qos = kp = ks = hk = ko = kos = 0
         if q is not None:
             if q_out is None:
                 q_out = _output(q, stream)
-            qs, qos, hq = _rows(q, None, hd, "q"), _rows(q_out, q.shape[1], hd, "q_out"), q.shape[1]
+            qs, hq = _rows(q, None, hd, "q", dev), q.shape[1]
+            qos = _rows(q_out, hq, hd, "q_out", dev)
             qp, qo = q.data_ptr(), q_out.data_ptr()
             if q_out.dtype is not q.dtype or q_out.shape[0] != n:
                 raise ValueError("q and its output must have one type and number of tokens")
         if k is not None:
             if k_out is None:
                 k_out = _output(k, stream)
-            ks, kos, hk = _rows(k, None, hd, "k"), _rows(k_out, k.shape[1], hd, "k_out"), k.shape[1]
+            ks, (nk, hk, _) = _rows(k, None, hd, "k", dev), k.shape
+            kos = _rows(k_out, hk, hd, "k_out", dev)
             kp, ko = k.data_ptr(), k_out.data_ptr()
-            if k_out.dtype is not k.dtype or k_out.shape[0] != n or k.shape[0] != n or k.dtype is not t.dtype:
+            if k_out.dtype is not k.dtype or k_out.shape[0] != n or nk != n or k.dtype is not t.dtype:
                 raise ValueError("q, k and their outputs must have one type and number of tokens")
         rc = self._call(self._ref, pos.data_ptr(), n, qp, qs, hq, qo, qos, kp, ks, hk, ko, kos,
                         0 if t is None else _dtype(t), 1 if inverse else 0, 0 if stream is None else stream.cuda_stream)
@@ -117,7 +123,9 @@ class Q8Batch:
             if t is not None and (t.dtype != torch.int32 or tuple(t.shape) != (size,) or not t.is_contiguous()
                                   or not t.is_cuda):
                 raise ValueError(f"{name} must be a contiguous int32 CUDA tensor [{size}]")
-        self._keep = (cu, kv_len, seq)
+            if t is not None and t.get_device() != cu.get_device():
+                raise ValueError(f"{name} is on device {t.get_device()}, cu on {cu.get_device()}")
+        self._keep, self.device = (cu, kv_len, seq), cu.get_device()
         self.n_tokens = n_tokens
         self.b = SpQ8Batch(n, n_tokens, max_new, max_kv, _ptr(seq), cu.data_ptr(), kv_len.data_ptr())
         self.ref = C.byref(self.b)
@@ -135,7 +143,7 @@ class Q8Cache:
         check(lib().sp_cuda_q8_cache_init(C.byref(self.qc), C.byref(cfg), _FORMATS[fmt], block_tokens, n_seqs,
                                           max_seq_len, _stream_ptr(stream)), "sp_cuda_q8_cache_init")
         self.head_dim, self.n_layers, self.n_heads_kv, self.n_seqs = head_dim, n_layers, n_heads_kv, n_seqs
-        self.block_tokens, self.max_seq_len = block_tokens, self.qc.max_seq_len
+        self.block_tokens, self.max_seq_len, self.device = block_tokens, self.qc.max_seq_len, self.qc.device
         self._ref = C.byref(self.qc)
         self._write, self._read, self._attn = (lib().sp_cuda_q8_write_kv_tokens, lib().sp_cuda_q8_read_kv_tokens,
                                                lib().sp_cuda_q8_attn)
@@ -172,12 +180,14 @@ class Q8Cache:
         t = v if k is None else k
         if t is None:
             return
-        stride = _rows(t, self.n_heads_kv, self.head_dim, "k")
+        stride = _rows(t, self.n_heads_kv, self.head_dim, "k", self.device)
         if k is not None and v is not None and (v.dtype is not k.dtype or v.shape[0] != k.shape[0]
-                                                or _rows(v, self.n_heads_kv, self.head_dim, "v") != stride):
+                                                or _rows(v, self.n_heads_kv, self.head_dim, "v", self.device) != stride):
             raise ValueError("k and v must have one type, token stride and number of tokens")
         if t.shape[0] != batch.n_tokens:
             raise ValueError(f"{t.shape[0]} tokens, the batch has {batch.n_tokens}")
+        if batch.device != self.device:
+            raise ValueError(f"the batch is on device {batch.device}, the cache on {self.device}")
         rc = self._write(self._ref, layer, batch.ref, 0 if k is None else k.data_ptr(), 0 if v is None else v.data_ptr(),
                          stride, _dtype(t))
         if rc:
@@ -185,7 +195,7 @@ class Q8Cache:
 
     def read_kv_tokens(self, which: int, layer: int, seq: int, start_pos: int, out) -> None:
         """out: [n_tok][n_heads_kv][head_dim], contiguous (f32/f16/bf16)."""
-        if _rows(out, self.n_heads_kv, self.head_dim, "out") != 0:
+        if _rows(out, self.n_heads_kv, self.head_dim, "out", self.device) != 0:
             raise ValueError(f"out must be contiguous [tokens][{self.n_heads_kv}][{self.head_dim}]")
         rc = self._read(self._ref, which, layer, seq, start_pos, out.shape[0], out.data_ptr(), _dtype(out))
         if rc:
@@ -198,14 +208,16 @@ class Q8Cache:
         n, hq, hd = *q.shape[:2], self.head_dim
         if out is None:
             out = _output(q, stream)
-        qs, os = _rows(q, None, hd, "q"), _rows(out, hq, hd, "out")
+        qs, os = _rows(q, None, hd, "q", self.device), _rows(out, hq, hd, "out", self.device)
         if n != batch.n_tokens or out.shape[0] != n or out.dtype is not q.dtype:
             raise ValueError(f"q and out must have one type and the batch's {batch.n_tokens} tokens")
+        if batch.device != self.device:
+            raise ValueError(f"the batch is on device {batch.device}, the cache on {self.device}")
         lp = 0
         if lse is not None:
-            if lse.shape != (n, hq) or lse.element_size() != 4 or not (lse.is_floating_point() and lse.is_cuda
-                                                                       and lse.is_contiguous()):
-                raise ValueError(f"lse must be a contiguous float32 CUDA tensor [{n}][{hq}]")
+            if lse.shape != (n, hq) or lse.element_size() != 4 or not (lse.is_floating_point() and lse.is_contiguous()
+                                                                       and lse.get_device() == self.device):
+                raise ValueError(f"lse must be a contiguous float32 tensor [{n}][{hq}] on device {self.device}")
             lp = lse.data_ptr()
         rc = self._attn(self._ref, layer, batch.ref, q.data_ptr(), qs, hq, _dtype(q), logit_scale, 1 if causal else 0, window,
                         out.data_ptr(), os, lp, 0 if stream is None else stream.cuda_stream)

@@ -24,7 +24,7 @@ def _cache(hd=64, heads=2):
     import spb200
     c = object.__new__(spb200.Q8Cache)
     c.qc = spb200.SpQ8Cache()
-    c.head_dim, c.n_heads_kv, c.fmt, c.stream = hd, heads, "int8", None
+    c.head_dim, c.n_heads_kv, c.fmt, c.stream, c.device = hd, heads, "int8", None, 0
     c._ref = None
 
     def launched(*a):
@@ -38,6 +38,11 @@ def _batch(n_tokens):
     b = object.__new__(spb200.Q8Batch)
     b._keep, b.n_tokens, b.ref, b.device = (), n_tokens, None, 0
     return b
+
+
+@pytest.fixture(autouse=True)
+def current_device(monkeypatch):
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
 
 
 def _rope():
@@ -92,3 +97,32 @@ def test_runs_of_more_tiles_than_32_bits_count(tmp_path):
     subprocess.run([b.HOST_CXX, "-O1", "-std=c++17", "-Wall", "-Werror", f"-I{PKG / 'csrc'}",
                     str(ROOT / "tests" / "c" / "q8_runs_check.cpp"), "-o", str(exe)], check=True)
     assert subprocess.run([str(exe)], capture_output=True, text=True).stdout == "ok\n"
+
+
+def test_tensors_of_another_device_are_refused(built_lib):
+    """Pointers of another card's memory are none of the kernels'."""
+    import spb200
+    rope, pos = _rope()
+    cache, batch = _cache(), _batch(5)
+    far, here = OnCard(_all().t, device=1), _all()
+    lse = OnCard(torch.zeros(5, 2), device=1)
+    other = _batch(5)
+    other.device = 1
+    out = OnCard(torch.zeros(5, 2, 64, dtype=torch.float16), device=1)
+    for call in (lambda: rope.apply(pos, far, None, q_out=here), lambda: rope.apply(pos, here, None, q_out=far),
+                 lambda: rope.apply(pos, None, far, k_out=here), lambda: rope.apply(pos, None, here, k_out=far),
+                 lambda: rope.apply(OnCard(pos.t, device=1), far, None, q_out=far),
+                 lambda: cache.write_kv_tokens(0, batch, far, far), lambda: cache.write_kv_tokens(0, batch, here, far),
+                 lambda: cache.write_kv_tokens(0, batch, None, far), lambda: cache.write_kv_tokens(0, other, here, here),
+                 lambda: cache.read_kv_tokens(0, 0, 0, 0, out), lambda: cache.attn(0, batch, far, out=here),
+                 lambda: cache.attn(0, batch, here, out=far), lambda: cache.attn(0, other, here, out=here),
+                 lambda: cache.attn(0, batch, here, out=here, lse=lse)):
+        with pytest.raises(ValueError, match="device"):
+            call()
+    cu, kv = OnCard(torch.zeros(3, dtype=torch.int32)), OnCard(torch.zeros(2, dtype=torch.int32), device=1)
+    with pytest.raises(ValueError, match="device"):
+        spb200.Q8Batch(cu, kv, 4, 4, 4)
+    with pytest.raises(AssertionError):          # the same on the right card reaches the library
+        rope.apply(pos, here, here, q_out=here, k_out=here)
+    with pytest.raises(AssertionError):
+        cache.attn(0, batch, here, out=here, lse=OnCard(lse.t))
