@@ -59,6 +59,35 @@ def _output(t, stream):
     return out
 
 
+_ROTATION = None
+
+
+def _rotation():
+    """The rotation as a function with a gradient, which is the rotation back."""
+    global _ROTATION
+    if _ROTATION is None:
+        import torch
+
+        class Rotation(torch.autograd.Function):
+            @staticmethod
+            def forward(ctx, plan, pos, q, k, inverse, stream):
+                ctx.plan, ctx.inverse = plan, inverse
+                ctx.save_for_backward(pos)
+                out = plan.apply(pos, q, k, inverse=inverse, stream=stream)
+                ctx.mark_non_differentiable(*(t for t, need in zip(out, ctx.needs_input_grad[2:4]) if t is not None and not need))
+                return out
+
+            @staticmethod
+            def backward(ctx, gq, gk):
+                pos, = ctx.saved_tensors
+                gq, gk = (g.contiguous() if g is not None and need else None
+                          for g, need in zip((gq, gk), ctx.needs_input_grad[2:4]))
+                gq, gk = ctx.plan.apply(pos, gq, gk, inverse=not ctx.inverse, stream=torch.cuda.current_stream(pos.device))
+                return None, None, gq, gk, None, None
+        _ROTATION = Rotation
+    return _ROTATION
+
+
 class RopeAxes:
     """A rotation plan: `sections` pairs for each axis (together rot_dim / 2)."""
 
@@ -74,12 +103,18 @@ class RopeAxes:
         self.head_dim, self.n_axes = head_dim, len(sections)
         import torch
         self._ref, self._call = C.byref(self.plan), lib().sp_cuda_rope_axes
-        self._int32, self._device = torch.int32, torch.cuda.current_device      # a step's call is host time
+        # a step's call is host time
+        self._int32, self._device, self._grad_enabled = torch.int32, torch.cuda.current_device, torch.is_grad_enabled
 
     def apply(self, pos, q=None, k=None, q_out=None, k_out=None, inverse: bool = False, stream=None):
         """Rotates q and k ([tokens][heads][head_dim] CUDA tensors; either may be
         None) at positions pos (int32 [axes][tokens]).  The outputs are new
-        tensors unless given; an output may be its input.  Returns both."""
+        tensors unless given; an output may be its input.  Returns both.  Where
+        gradients are wanted they flow back through it, and outputs cannot be given."""
+        if (q is not None and q.requires_grad or k is not None and k.requires_grad) and self._grad_enabled():
+            if q_out is not None or k_out is not None:
+                raise RuntimeError("a rotation into a given output has no gradient: leave the output out, or use torch.no_grad()")
+            return _rotation().apply(self, pos, q, k, inverse, stream)
         t = k if q is None else q
         n, dev = 0 if t is None else t.shape[0], pos.get_device()
         if pos.dtype is not self._int32 or pos.shape != (self.n_axes, n) or dev < 0 or not pos.is_contiguous():
@@ -204,7 +239,8 @@ class Q8Cache:
     def attn(self, layer: int, batch: Q8Batch, q, out=None, lse=None, logit_scale: float = 1.0, causal: bool = True,
              window: int = 0, stream=None):
         """q: [n_tokens][n_q_heads][head_dim] fp16 or bf16; out the same (new unless
-        given); lse: fp32 [n_tokens][n_q_heads] or None.  Returns out."""
+        given); lse: fp32 [n_tokens][n_q_heads] or None.  Returns out, which has
+        no gradient."""
         n, hq, hd = *q.shape[:2], self.head_dim
         if out is None:
             out = _output(q, stream)

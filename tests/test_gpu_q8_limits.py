@@ -167,3 +167,70 @@ def test_new_outputs_are_memory_of_their_stream(cuda, which):
             assert y.data_ptr() != at
             torch.cuda.synchronize()
             assert torch.equal(w, y)
+
+
+# ------------------------------------------------------------------ gradients --
+
+@pytest.mark.parametrize("pairing", ["adjacent", "halves"])
+@pytest.mark.parametrize("inverse", [False, True])
+def test_rope_autograd(cuda, pairing, inverse):
+    """The gradient of q and k (slices of one projection) against autograd through the
+    formula in 64 bits, and against differences of the loss."""
+    T, hq, hk, hd, rot = 23, 5, 2, 64, 48
+    plan = spb200.RopeAxes(hd, [8, 8, 8], pairing=pairing, rot_dim=rot)
+    g = torch.Generator(device="cuda").manual_seed(6)
+    pos = torch.randint(0, 9000, (3, T), generator=g, device="cuda", dtype=torch.int32)
+    x = torch.randn(T, hq + hk, hd, generator=g, device="cuda", requires_grad=True)
+    w = torch.randn(T, hq + hk, hd, generator=g, device="cuda")
+
+    def loss(z):
+        q, k = plan.apply(pos, z[:, :hq], z[:, hq:], inverse=inverse)
+        return (torch.cat([q, k], 1).double() * w.double()).sum()
+    grad, = torch.autograd.grad(loss(x), x)
+    # the formula, its cosines as constants
+    f = torch.tensor([float(np.float32(10000.0 ** (-2.0 * i / rot))) for i in range(rot // 2)], dtype=torch.float64, device="cuda")
+    axis = torch.arange(3, device="cuda").repeat_interleave(8)
+    a = (pos[axis].double().t() * f)[:, None] * (-1.0 if inverse else 1.0)
+    z = x.detach().double().requires_grad_()
+    u, v = (z[..., 0:rot:2], z[..., 1:rot:2]) if pairing == "adjacent" else (z[..., :rot // 2], z[..., rot // 2:rot])
+    lo, hi = u * a.cos() - v * a.sin(), u * a.sin() + v * a.cos()
+    y = torch.stack([lo, hi], -1).flatten(-2) if pairing == "adjacent" else torch.cat([lo, hi], -1)
+    want, = torch.autograd.grad((torch.cat([y, z[..., rot:]], -1) * w.double()).sum(), z)
+    # each element is a rotation of a pair of w: its rounding and the cosines' (4e-7 of the pair's length)
+    assert ((grad.double() - want).abs() <= 6e-7 * (w.double().abs().amax() * 2 ** 0.5)).all()
+    d = torch.randn(x.shape, generator=g, device="cuda")
+    step = 2.0 ** -3            # the loss is linear: a large step only rounds less
+    with torch.no_grad():
+        numeric = ((loss(x + step * d) - loss(x - step * d)) / (2 * step)).item()
+    size = w.double().norm().item() * (x.detach().double().norm().item() / step + d.double().norm().item())
+    assert abs(numeric - (grad.double() * d.double()).sum().item()) <= 4e-7 * size
+
+
+def test_rope_autograd_shapes_and_streams(cuda):
+    """One half alone, a half without a gradient, a gradient expanded from one number,
+    a second derivative, another stream, and nothing kept without gradients."""
+    T, hd = 9, 64
+    plan = spb200.RopeAxes(hd, [32])
+    pos = torch.arange(T, dtype=torch.int32, device="cuda")[None]
+    x = torch.randn(T, 3, hd, device="cuda", requires_grad=True)
+    k = torch.randn(T, 1, hd, device="cuda")
+    back = plan.apply(pos, torch.ones_like(k), None, inverse=True)[0].expand(T, 3, hd)
+    for q, kk in ((x, None), (None, x), (x, k), (k, x)):
+        y = plan.apply(pos, q, kk)
+        mine = y[0] if q is x else y[1]
+        assert mine.requires_grad and not any(o.requires_grad for o in y if o is not None and o is not mine)
+        grad, = torch.autograd.grad(mine.sum(), x)
+        assert torch.equal(grad, back)
+    y = plan.apply(pos, x, None)[0]
+    grad, = torch.autograd.grad(y.square().sum(), x, create_graph=True)      # 2 x, whose own derivative is 2
+    again, = torch.autograd.grad(grad.sum(), x)
+    assert ((again - 2.0).abs() <= 2e-6 * 4).all()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        grad, = torch.autograd.grad(plan.apply(pos, x, None, stream=side)[0].sum(), x)
+    side.synchronize()
+    assert torch.equal(grad, back)
+    with torch.no_grad():
+        assert not plan.apply(pos, x, None)[0].requires_grad
+    assert not plan.apply(pos, x.detach(), None)[0].requires_grad

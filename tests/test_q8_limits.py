@@ -126,3 +126,16 @@ def test_tensors_of_another_device_are_refused(built_lib):
         rope.apply(pos, here, here, q_out=here, k_out=here)
     with pytest.raises(AssertionError):
         cache.attn(0, batch, here, out=here, lse=OnCard(lse.t))
+
+
+def test_rotation_that_would_lose_a_gradient_is_refused(built_lib):
+    """With gradients wanted an output cannot be given; without them it can."""
+    rope, pos = _rope()
+    x = OnCard(torch.zeros(5, 2, 64, requires_grad=True))
+    out = OnCard(torch.zeros(5, 2, 64))
+    for call in (lambda: rope.apply(pos, x, None, q_out=out), lambda: rope.apply(pos, None, x, k_out=out),
+                 lambda: rope.apply(pos, out, x, q_out=out, k_out=out), lambda: rope.apply(pos, x, None, q_out=x)):
+        with pytest.raises(RuntimeError, match="gradient"):
+            call()
+        with torch.no_grad(), pytest.raises(AssertionError, match="reached"):
+            call()
