@@ -43,10 +43,7 @@ extern "C" int sp_rope_axes_init(sp_rope_axes_t *ra, int head_dim, int rot_dim, 
     if (sum != n_pairs)
         return sp_set_error(SP_ERR_ARG, "rope_axes_init: the sections have %lld pairs, rot_dim %d has %d", sum, rot_dim,
                             n_pairs);
-    ra->head_dim = head_dim;
-    ra->rot_dim = rot_dim;
-    ra->n_axes = n_axes;
-    ra->pairing = pairing;
+    sp_rope_axes_t plan = {head_dim, rot_dim, n_axes, pairing, {}, {}};      // *ra stays empty where a frequency is refused
     int used[SP_ROPE_MAX_AXES] = {0, 0, 0, 0};
     int a = 0;
     for (int i = 0; i < n_pairs; i++) {
@@ -63,11 +60,12 @@ extern "C" int sp_rope_axes_init(sp_rope_axes_t *ra, int head_dim, int rot_dim, 
         // whole turns for each step do not matter at whole positions
         double turn = f / 6.283185307179586476925;
         turn -= floor(turn);
-        ra->phase[i] = turn >= 1.0 ? 0 : (uint64_t)ldexp(turn, 64);
-        ra->axis[i] = (uint8_t)a;
+        plan.phase[i] = turn >= 1.0 ? 0 : (uint64_t)ldexp(turn, 64);
+        plan.axis[i] = (uint8_t)a;
         used[a]++;
         if (flags & SP_ROPE_INTERLEAVED) a = (a + 1) % n_axes;
     }
+    *ra = plan;
     return SP_OK;
 }
 

@@ -139,3 +139,19 @@ def test_rotation_that_would_lose_a_gradient_is_refused(built_lib):
             call()
         with torch.no_grad(), pytest.raises(AssertionError, match="reached"):
             call()
+
+
+def test_refused_plan_is_no_plan(built_lib):
+    """A plan whose frequencies were refused half-way, after one that was good."""
+    import ctypes as C
+
+    import spb200
+    L, plan = spb200.lib(), spb200.SpRopeAxes()
+
+    def init(factors):
+        return L.sp_rope_axes_init(C.byref(plan), 64, 64, 0, 1, (C.c_int * 1)(32), 0, 1e4, (C.c_float * 32)(*factors))
+    for bad in ([1.0] * 31 + [0.0], [1.0] * 20 + [1e-45] * 12, [float("inf")] + [1.0] * 31):
+        assert init([1.0] * 32) == 0 and plan.head_dim == 64
+        assert init(bad) == spb200.SP_ERR_ARG
+        assert bytes(plan) == bytes(C.sizeof(plan))
+        assert L.sp_cuda_rope_axes(C.byref(plan), None, 0, None, 0, 0, None, 0, None, 0, 0, None, 0, 1, 0, None) == spb200.SP_ERR_ARG
