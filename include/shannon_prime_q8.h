@@ -120,7 +120,9 @@ typedef struct {
  * are in device memory, so a step's graph can be replayed with other lengths.
  * Entry i is skipped, and bit 0 of the status word set, unless
  *     0 <= d_cu[i] <= d_cu[i+1] <= n_tokens, d_cu[i+1] - d_cu[i] <= max_new,
- *     0 <= d_kv_len[i] <= max_kv, 0 <= d_seq[i] < n_seqs of the cache. */
+ *     0 <= d_kv_len[i] <= max_kv, 0 <= d_seq[i] < n_seqs of the cache.
+ * No two entries share packed tokens.  Where d_cu descends (which sets bit 0) they
+ * may, and a write may then leave blocks out that come after n_tokens' worth. */
 typedef struct {
     int        n_seqs;     /* entries, any number >= 0 */
     int        n_tokens;   /* packed tokens of all entries */
@@ -171,9 +173,10 @@ int  sp_cuda_q8_read_kv_tokens(const sp_cuda_q8_cache_t *qc, int which, int laye
  *               reads KV head g / (n_q_heads / n_heads_kv)
  *   d_lse       NULL or fp32 [n_tokens][n_q_heads]: log sum_j exp(logit_scale q.K[j]),
  *               to join this result with attention over other positions
- * Scores, the softmax's statistics and sums are held in 32 bits; softmax
- * weights are rounded to 16 bits (fp16, relative to a running maximum) for the
- * product with V.  Calls on one cache must not overlap on the GPU (they share
+ * Scores, the softmax's statistics and sums are held in 32 bits; queries are
+ * rounded to fp16 after a power of two that brings a row's largest element to
+ * [1, 2) (elements under 2^-14 of it lose bits), softmax weights to fp16,
+ * relative to a running maximum, for the product with V.  Calls on one cache must not overlap on the GPU (they share
  * its workspace). */
 int  sp_cuda_q8_attn(const sp_cuda_q8_cache_t *qc, int layer, const sp_cuda_q8_batch_t *batch,
                      const void *d_q, long long q_stride, int n_q_heads, int dtype,
