@@ -24,7 +24,10 @@
 // 3900 cycles, the products 2100 of them.  Tensor memory is full (two scores,
 // two outputs), so the next scores cannot be computed earlier: in halves of 64
 // columns, one of them ahead, the prompt took 994 us, since products of 64
-// columns cost 3/4 of those of 128.  The beginning and end of a unit (queries,
+// columns cost 3/4 of those of 128.  The same prompt in 64 dimensions takes 559
+// us, 490 TFLOP/s: products are half as long, the rest of the chain is not, and the
+// powers of two alone keep the special-function units busy for 231 us (the
+// polynomial takes an eighth of them).  The beginning and end of a unit (queries,
 // output) take about 12000 cycles, a tenth of the prompt's time.
 #include "sp_q8_attn.cuh"
 #include "sp_q8_runs.h"
