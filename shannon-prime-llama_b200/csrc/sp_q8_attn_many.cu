@@ -98,6 +98,13 @@ __device__ __forceinline__ void tmem_ld16(uint32_t at, uint32_t (&v)[16])
                    "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
                  : "r"(at));
 }
+// With its wait.
+__device__ __forceinline__ void tmem_ld8(uint32_t at, uint32_t (&v)[8])
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n\ttcgen05.wait::ld.sync.aligned;"
+                 : "=&r"(v[0]), "=&r"(v[1]), "=&r"(v[2]), "=&r"(v[3]), "=&r"(v[4]), "=&r"(v[5]), "=&r"(v[6]), "=&r"(v[7])
+                 : "r"(at) : "memory");
+}
 __device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t (&v)[16])
 {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
@@ -528,7 +535,7 @@ __global__ void __launch_bounds__(Shape<HD>::Threads, 1) k_q8_attn_many(const __
                 };
                 // ---- the same where positions are masked or the maximum has to grow: it is
                 // found first, and what the products so far have summed, and this tile's
-                // weights before these, shrink.
+                // weights before these (rounded a second time), shrink.
                 auto careful = [&](int c) {
                     float top = kNone;
 #pragma unroll 1
@@ -562,18 +569,20 @@ __global__ void __launch_bounds__(Shape<HD>::Threads, 1) k_q8_attn_many(const __
                             }
                         }
                         wait_st();
-                        const __half2 x = __float2half2_rn(fix);
+                        // in 32 bits: fix may be far below fp16's normal numbers, and
+                        // the weights as far above 1 (up to 2^12).  8 columns at a time:
+                        // 16 take the kernel from 122 registers to 128
 #pragma unroll 1
-                        for (int d = 0; d < 16 * c; d += 16) {
-                            uint32_t v[16];
-                            tmem_ld16(t_s + d, v);
-                            wait_ld16(v);
+                        for (int d = 0; d < 16 * c; d += 8) {
+                            uint32_t v[8];
+                            tmem_ld8(t_s + d, v);
 #pragma unroll
-                            for (int j = 0; j < 16; j++) {
-                                const __half2 y = __hmul2(*reinterpret_cast<const __half2 *>(&v[j]), x);
-                                v[j] = *reinterpret_cast<const uint32_t *>(&y);
+                            for (int j = 0; j < 8; j++) {
+                                const float2 y = __half22float2(*reinterpret_cast<const __half2 *>(&v[j]));
+                                const __half2 z = __floats2half2_rn(y.x * fix, y.y * fix);
+                                v[j] = *reinterpret_cast<const uint32_t *>(&z);
                             }
-                            tmem_st16(t_s + d, v);
+                            tmem_st8(t_s + d, v);
                         }
                     }
 #pragma unroll 1

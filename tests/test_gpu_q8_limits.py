@@ -107,6 +107,42 @@ def test_attn_nan_queries_other_dims(cuda, hd, new, kv):
                     0.1, True, 0)
 
 
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("fmt,dtype", [("int8", "f16"), ("e4m3", "bf16")])
+def test_attn_maximum_rises_inside_a_tile(cuda, hd, fmt, dtype):
+    """A key 2^9 to 2^11.5 times the others' weight, then, up to 63 positions on, one that
+    takes nearly all of it and has no value: what the first one leaves in the output
+    is its weight rounded at most twice to fp16 (2^-11 of it, or 2^-25 of the largest)."""
+    seqs, H, G, B, n, new = 32, 8, 4, 64, 600, 40       # more tiles than CTAs by far: runs of many tiles
+    cache = spb200.Q8Cache(hd, 1, H, n, n_seqs=seqs, fmt=fmt, block_tokens=B)
+    g = torch.Generator().manual_seed(12)
+    u = torch.randint(0, 2, (hd,), generator=g).float() * 2 - 1
+    kc, vc = torch.zeros(seqs, H, cache.max_seq_len, hd), torch.zeros(seqs, H, cache.max_seq_len, hd)
+    for i in range(seqs):
+        first = 256 + (5 * i) % 32
+        kc[i, :, first], kc[i, :, 256 + 32 + (3 * i) % 32] = 64.0 * u, 112.0 * u
+        vc[i, :, first] = torch.randint(1, 8, (H, hd), generator=g).float() * 16
+    for which, c, s in ((0, kc, 2.0 ** -7), (1, vc, 2.0 ** -5)):
+        cache.slab(which).view(torch.uint8).copy_(R.code(c, fmt).view(1, *c.shape))
+        cache.scales(which).fill_(s)
+    q = (u + 0.25 * torch.randn(seqs * new, H * G, hd, generator=g)).to(R.DTYPES[dtype]).cuda()
+    out, lse = torch.empty_like(q), torch.empty(seqs * new, H * G, device="cuda")
+    qd = q.double().view(seqs, new, H, G, hd)
+    raw = torch.einsum("stkgd,sknd->stkgn", qd, kc[:, :, :n].double().cuda() * 2.0 ** -7)
+    seen = torch.arange(n, device="cuda")[None] <= torch.arange(n - new, n, device="cuda")[:, None]
+    for rise in (9.0, 10.0, 10.7, 11.5):
+        scale = rise * np.log(2.0) / (64.0 * hd / 128)
+        cache.attn(0, _batch([new] * seqs, [n] * seqs), q, out=out, lse=lse, logit_scale=scale)
+        assert cache.status() == 0
+        z = torch.where(seen[None, :, None, None], raw * scale, -torch.inf)
+        want = torch.einsum("stkgn,sknd->stkgd", torch.softmax(z, -1), vc[:, :, :n].double().cuda() * 2.0 ** -5).reshape(out.shape)
+        size = (qd.abs().sum(-1).max() * 112 * 2.0 ** -7 * scale).item()
+        tol = (R.EPS[dtype] + 2 * 2.0 ** -11 + 2.0 ** -18 * (1 + size)) * want.abs() + 2 * 2.0 ** -25 * 7 * 16 * 2.0 ** -5
+        off = (out.double() - want).abs()
+        assert (off <= tol).all(), (rise, (off / tol).max().item())
+        assert ((lse.double() - torch.logsumexp(z, -1).reshape(lse.shape)).abs() <= 2.0 ** -18 * (1 + size)).all()
+
+
 # -------------------------------------------------------- windows and tokens --
 
 @pytest.mark.parametrize("hd", [64, 128, 256])
