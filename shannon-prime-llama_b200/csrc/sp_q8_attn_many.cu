@@ -535,7 +535,10 @@ __global__ void __launch_bounds__(Shape<HD>::Threads, 1) k_q8_attn_many(const __
                 };
                 // ---- the same where positions are masked or the maximum has to grow: it is
                 // found first, and what the products so far have summed, and this tile's
-                // weights before these (rounded a second time), shrink.
+                // weights before these (rounded a second time), shrink.  Exponents are
+                // differences of the numbers that the maximum was taken of: in one sum with
+                // scale and maximum, as above, the largest key's own is off by as much as the
+                // maximum was rounded, 2^5 at logits of 1e9.
                 auto careful = [&](int c) {
                     float top = kNone;
 #pragma unroll 1
@@ -587,7 +590,7 @@ __global__ void __launch_bounds__(Shape<HD>::Threads, 1) k_q8_attn_many(const __
                     }
 #pragma unroll 1
                     for (int h = 2 * c; h < 2 * c + 2; h++) {
-                        const float fg = sc[h].x * mul, off = sc[h].y - m;
+                        const float fg = sc[h].x * mul, lg = sc[h].y;
                         uint32_t v[16], p[8];
                         tmem_ld16(t_s + 16 * h, v);
                         wait_ld16(v);
@@ -595,8 +598,8 @@ __global__ void __launch_bounds__(Shape<HD>::Threads, 1) k_q8_attn_many(const __
 #pragma unroll
                         for (int j = 0; j < 16; j += 2) {
                             const int at = j0 + 16 * h + j;
-                            const float x = at > hi || at < lo ? 0.0f : ex2(fmaf(__uint_as_float(v[j]), fg, off));
-                            const float y = at + 1 > hi || at + 1 < lo ? 0.0f : ex2(fmaf(__uint_as_float(v[j + 1]), fg, off));
+                            const float x = at > hi || at < lo ? 0.0f : ex2(fmaf(__uint_as_float(v[j]), fg, lg) - m);
+                            const float y = at + 1 > hi || at + 1 < lo ? 0.0f : ex2(fmaf(__uint_as_float(v[j + 1]), fg, lg) - m);
                             sum += x + y;
                             const __half2 hw = __floats2half2_rn(x, y);
                             p[j / 2] = *reinterpret_cast<const uint32_t *>(&hw);

@@ -143,6 +143,44 @@ def test_attn_maximum_rises_inside_a_tile(cuda, hd, fmt, dtype):
         assert ((lse.double() - torch.logsumexp(z, -1).reshape(lse.shape)).abs() <= 2.0 ** -18 * (1 + size)).all()
 
 
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("fmt,dtype", [("int8", "f16"), ("e4m3", "bf16")])
+@pytest.mark.parametrize("new", [2, 40])
+def test_attn_logits_past_32_bit_resolution(cuda, hd, fmt, dtype, new):
+    """Logits of 1e7 to 1e30, whose neighbours are whole numbers of powers of two apart: the key
+    that is far above the others, at each position mod 32, is the output."""
+    H, G, B, n, seqs = 1, 4, 64, 600, 32
+    cache = spb200.Q8Cache(hd, 1, H, n, n_seqs=seqs, fmt=fmt, block_tokens=B)
+    kc, ks, vc, vs = _fill(cache, 31)
+    g = torch.Generator().manual_seed(8)
+    u = torch.randint(0, 2, (hd,), generator=g).float() * 2 - 1
+    kc.copy_(R.code(torch.randn(kc.shape, generator=g) * 2.5, fmt).view(kc.shape))
+    ks.fill_(2.0 ** -7)
+    at = [32 * (5 * i % 17) + i for i in range(seqs)]
+    for i, j in enumerate(at):
+        kc[0, i, 0, j] = R.code(112.0 * u, fmt)
+    for which, c, s in ((0, kc, ks), (1, vc, vs)):
+        cache.slab(which).view(torch.uint8).copy_(c)
+        cache.scales(which).copy_(s)
+    q = u + 0.25 * torch.randn(seqs * new, G, hd, generator=g)
+    q = q.to(R.DTYPES[dtype])
+    out, lse = torch.empty(seqs * new, G, hd, device="cuda", dtype=q.dtype), torch.empty(seqs * new, G, device="cuda")
+    for causal in (True, False):
+        for size in (1e7, 1e8, 1e9, 1e12, 1e30):
+            scale = size / (112.0 * hd / 128)
+            cache.attn(0, _batch([new] * seqs, [n] * seqs), q.cuda(), out=out, lse=lse, logit_scale=scale, causal=causal)
+            assert cache.status() == 0
+            for i, j in enumerate(at):
+                rows = slice(i * new, i * new + new)
+                want = R.values(vc[0, i, 0, j], fmt).double() * vs[0, i, 0, j // B].double()
+                off = (out[rows].double().cpu() - want).abs()
+                # the output's rounding, the weight's, and the sum's reciprocal
+                assert (off <= (R.EPS[dtype] + 2.0 ** -11 + 2.0 ** -20) * want.abs() + 2.0 ** -25).all(), (size, i)
+                z = q[rows].double() @ (R.values(kc[0, i, 0, j], fmt).double() * 2.0 ** -7) * scale
+                # the scale's, the factors' and the sum's roundings
+                assert ((lse[rows].double().cpu() - z).abs() <= 2.0 ** -19 * z.abs()).all(), (size, i)
+
+
 # -------------------------------------------------------- windows and tokens --
 
 @pytest.mark.parametrize("hd", [64, 128, 256])
