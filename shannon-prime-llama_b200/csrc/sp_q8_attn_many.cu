@@ -15,7 +15,7 @@
 // its 128 rows, the tensor cores work on the other 128.
 //
 // Measured: a causal prompt of 8192 tokens, 32 query heads on 8 of 128
-// dimensions, e4m3 and bf16, takes 705 us, 780 TFLOP/s (47% of the library's
+// dimensions, e4m3 and bf16, takes 711 us, 773 TFLOP/s (47% of the library's
 // plain product); chunks of 202 to 1021 tokens on up to 7570 positions, 16 query
 // heads on 2 of 256, int8, window 4096, 270 us, 685 TFLOP/s.  What bounds it is
 // the chain of a 128-row tile: scores, softmax (one row a thread, about 1950
@@ -24,10 +24,10 @@
 // 3900 cycles, the products 2100 of them.  Tensor memory is full (two scores,
 // two outputs), so the next scores cannot be computed earlier: in halves of 64
 // columns, one of them ahead, the prompt took 994 us, since products of 64
-// columns cost 3/4 of those of 128.  The same prompt in 64 dimensions takes 559
-// us, 490 TFLOP/s: products are half as long, the rest of the chain is not, and the
-// powers of two alone keep the special-function units busy for 231 us (the
-// polynomial takes an eighth of them).  The beginning and end of a unit (queries,
+// columns cost 3/4 of those of 128.  The same prompt in 64 dimensions takes 577
+// us, 476 TFLOP/s: products are half as long, the rest of the chain is not, and the
+// powers of two alone keep the special-function units busy for 231 us (a polynomial
+// for a quarter or an eighth of them changed nothing).  The beginning and end of a unit (queries,
 // output) take about 12000 cycles, a tenth of the prompt's time.
 #include "sp_q8_attn.cuh"
 #include "sp_q8_runs.h"
@@ -149,26 +149,6 @@ __device__ __forceinline__ F2 add2(F2 a, F2 b)
         : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
     return d;
 }
-// 2^x for x in [-126, 126] (below: 2^-126; above, and for NaN: 2^126, which the
-// test for too small a maximum sees) without the special-function unit: the
-// nearest whole number n by adding and taking off 1.5 * 2^23, whose low bits
-// then are n and go to the exponent, which would wrap outside those limits;
-// 2^(x - n) by the polynomial of degree 4 with the least largest relative error
-// on [-1/2, 1/2], 2.7e-6 (Remez exchange).
-__device__ __forceinline__ F2 exp2_poly(F2 x)
-{
-    constexpr float kRound = 12582912.0f;
-    x.x = fmaxf(fminf(x.x, 126.0f), -126.0f);
-    x.y = fmaxf(fminf(x.y, 126.0f), -126.0f);
-    const F2 t = add2(x, {kRound, kRound}), n = add2(t, {-kRound, -kRound}), r = fma2(n, {-1.0f, -1.0f}, x);
-    F2 p = fma2({0x1.3997d6p-7f, 0x1.3997d6p-7f}, r, {0x1.ca1444p-5f, 0x1.ca1444p-5f});
-    p = fma2(p, r, {0x1.ec06dap-3f, 0x1.ec06dap-3f});
-    p = fma2(p, r, {0x1.62e0dcp-1f, 0x1.62e0dcp-1f});
-    p = fma2(p, r, {0x1.ffffe8p-1f, 0x1.ffffe8p-1f});
-    return {__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)),
-            __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23))};
-}
-
 // Shared-memory operand without swizzle, in core matrices of 8 rows of 16
 // bytes: lbo bytes between core matrices along K, sbo along M or N (for both
 // the K-major and the MN-major operands).
@@ -295,13 +275,6 @@ struct Walk {
         r = rows_of<HD>(a, e, qt);
     }
 };
-
-// Which pairs of weights take the polynomial: one in eight at head_dim 64, whose
-// products are short, so that the special-function unit bounds a tile (a causal
-// prompt of 8192 with 32 heads on 8: 559 us; one in four 561, none 567; at 128
-// one in four makes no difference, 707 and 710, and half of the pairs take 735).
-template <int HD>
-__host__ __device__ constexpr bool kPoly(int j) { return HD == 64 && j % 8 == 3; }
 
 template <typename T, int FMT, int HD>
 __global__ void __launch_bounds__(Shape<HD>::Threads, 1) k_q8_attn_many(const __grid_constant__ AttnArgs a)
@@ -518,12 +491,8 @@ __global__ void __launch_bounds__(Shape<HD>::Threads, 1) k_q8_attn_many(const __
 #pragma unroll
                         for (int j = 8 * h; j < 8 * h + 8; j++) {
                             F2 x = fma2({__uint_as_float(u[2 * j]), __uint_as_float(u[2 * j + 1])}, {fg, fg}, {off, off});
-                            if (kPoly<HD>(j)) {
-                                x = exp2_poly(x);
-                            } else {
-                                x.x = ex2(x.x);
-                                x.y = ex2(x.y);
-                            }
+                            x.x = ex2(x.x);
+                            x.y = ex2(x.y);
                             part = add2(part, x);
                             const __half2 hw = __floats2half2_rn(x.x, x.y);
                             p[j] = *reinterpret_cast<const uint32_t *>(&hw);
